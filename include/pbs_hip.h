@@ -236,6 +236,46 @@ int pbs_rope_qk(const void* q, const void* k, const void* cos, const void* sin, 
                 int Hkv, int S, int head_dim, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t k_sb, int64_t k_sh,
                 int64_t k_ss, int64_t c_sb, int64_t c_ss, void* stream);
 
+/* A paged key-value cache.  A pool holds num_pages pages of page_size tokens (32, 64, 128 or 256) of Hkv heads; row b of page_table
+ * ((B, max_pages) int32, row stride table_sb) lists the pages of sequence b in order, and token t of it lies in page t / page_size.  Only the
+ * entries that a call's tokens reach are read; the tokens of an entry outside 0 .. num_pages - 1, and those behind max_pages, are not
+ * stored, count as not there for the attention, and are read as zeros.
+ *   kv_bits 16   k_pages (page, head, token, 128) bf16, v_pages (page, head, token / 8, 128, token % 8) bf16; no scales
+ *   kv_bits 4    e2m1 codes, the even channel in a byte's low half: k_pages (page, head, token, 64 bytes), v_pages
+ *                (page, head, token / 4, channel / 8, token % 4, 4 bytes); k_scale, v_scale (page, head, token / 32, channel / 32, token % 32)
+ *                bytes: the exponent of the power of two that the group's codes are multiples of, plus 127.  The smallest exponent is
+ *                taken with which no value is above 7 units, within -100 .. 125; a group with an infinity or NaN is held as NaN (255).
+ * Pages and scales contiguous and 16-byte aligned.  past_lens, new_lens: (B) int32 on the GPU, tokens of each sequence before the call and
+ * new ones (null: S each; clamped to 0 .. S).  At most 2^30 tokens a sequence.
+ *
+ * pbs_paged_append: rotary embedding of q (B, Hq, S, 128) and k (B, Hkv, S, 128) in fp32 with one rounding to bf16 (cos and sin as in
+ * pbs_rope_qk; both null: no rotation), and k and v into the pages: row i < new_lens[b] at token past_lens[b] + i.  q with q_out, or both
+ * null.  k_out (null: not wanted) receives the rotated k.  q_out, k_out: contiguous, head-major, all S rows.  Sequences that share a page
+ * may read it, and at most one of them writes it.  Takes the place of pbs_attn/patch/huggingface.py:169-241 (embedding, then the
+ * cache's own update). */
+int pbs_paged_append(const void* q, const void* k, const void* v, const void* cos, const void* sin, void* q_out, void* k_out, void* k_pages,
+                     void* v_pages, void* k_scale, void* v_scale, const int32_t* page_table, const int32_t* past_lens,
+                     const int32_t* new_lens, int B, int Hq, int Hkv, int S, int head_dim, int num_pages, int max_pages, int page_size,
+                     int kv_bits, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sb,
+                     int64_t v_sh, int64_t v_ss, int64_t c_sb, int64_t c_ss, int64_t table_sb, void* stream);
+
+/* The first lens[b] tokens of every sequence as k_out, v_out (B, Hkv, max_len, 128) bf16, contiguous; rows from lens[b] on are zeros.  It has
+ * no counterpart in the reference. */
+int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, const int32_t* page_table,
+                   const int32_t* lens, void* k_out, void* v_out, int B, int Hkv, int max_len, int head_dim, int num_pages, int max_pages,
+                   int page_size, int kv_bits, int64_t table_sb, void* stream);
+
+/* Attention of the new tokens (appended before) over their sequences: query row i < new_lens[b] of q (B, Hq, S, 128) sees the tokens
+ * 0 .. past_lens[b] + i; out (B, Hq, S, 128) with its own strides.  Rows from new_lens[b] on, and rows whose keys weigh nothing, are zeros.
+ * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
+ * positive.  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
+size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len);
+int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                       const int32_t* page_table, const int32_t* past_lens, const int32_t* new_lens, void* out, int B, int Hq, int Hkv,
+                       int S, int head_dim, int num_pages, int max_pages, int page_size, int kv_bits, int max_len, int64_t q_sb,
+                       int64_t q_sh, int64_t q_ss, int64_t o_sb, int64_t o_sh, int64_t o_ss, int64_t table_sb, float softmax_scale,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,6 +3,7 @@ stream).  Tensors are bf16, head_dim 128, block_size 128; all outputs are
 allocated through torch's caching allocator."""
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -387,6 +388,125 @@ def rope_qk(q, k, cos, sin):
                                q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
                                c_sb, cos.stride(1), _stream()), "pbs_rope_qk")
     return q_out, k_out
+
+
+def _check_paged(pages, page_table, B, Hkv, lens, *ts):
+    """What every call on a paged cache checks; returns the arguments that describe the pages."""
+    _check_bf16_cuda(*ts)
+    k = pages.k
+    n, heads, page_size, _ = k.shape
+    device = k.device
+    if not k.is_cuda:
+        raise _lib.PbsHipError("PBS HIP kernels need tensors on the GPU (there is no CPU path)")
+    if heads != Hkv:
+        raise ValueError(f"pages of {heads} heads, K and V of {Hkv}")
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+        raise ValueError("page_table is (batch, pages of a sequence) int32, rows contiguous")
+    for t in lens:
+        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous()):
+            raise ValueError("lengths are (batch,) int32, contiguous")
+    for t in (*ts, page_table, *lens):
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {t.device} and pages on {device}")
+    return n, page_table.shape[1], page_size, 16 if pages.k_scale is None else 4
+
+
+def _on_device_of(t):
+    """The device of a call's tensors is made the current one, as the library's launches go there."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else _NO_SWITCH
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def paged_append(pages, page_table, past_lens, k, v, q=None, cos=None, sin=None, new_lens=None, want_k=False):
+    """New keys and values k, v (B, Hkv, S, 128) into the pages of a cache (``paged.KVPages``, written in place), rotated on the way:
+    row i of sequence b becomes its token ``past_lens[b] + i``, for the first ``new_lens[b]`` rows (None: all S).  Row b of
+    ``page_table`` (B, n) lists the pages of sequence b.  ``cos`` and ``sin`` (B or 1, S, 128) rotate q and k as ``rope_qk`` does,
+    with one rounding at the end; without them nothing is rotated.  All tensors on one GPU, lengths and table int32.
+    Returns (q, k) rotated, contiguous and head-major, all S rows: q (B, Hq, S, 128) where one is given, k with ``want_k``, else None.
+
+    Tokens whose page is not in the pool or that lie behind the table are not stored.  At most one sequence may write to a page."""
+    B, Hkv, S, D = k.shape
+    assert v.shape == k.shape and D == HEAD_DIM
+    assert q is None or (q.dim() == 4 and q.shape[0] == B and q.shape[2:] == (S, D))
+    if (cos is None) != (sin is None):
+        raise ValueError("cos goes with sin")
+    given = [t for t in (k, v, q, cos, sin) if t is not None]
+    n, max_pages, page_size, bits = _check_paged(pages, page_table, B, Hkv, (past_lens, new_lens), *given)
+    c_sb = c_ss = 0
+    if cos is not None:
+        assert cos.shape == sin.shape and cos.dim() == 3 and cos.shape[0] in (1, B) and cos.shape[1:] == (S, D)
+        cos, sin = _rows16(cos), _rows16(sin)
+        if cos.stride() != sin.stride():
+            cos, sin = cos.contiguous(), sin.contiguous()
+        c_sb, c_ss = cos.stride(0) if cos.shape[0] > 1 else 0, cos.stride(1)
+    k, k_ptr, k_strides = _rows16_args(k)
+    v, v_ptr, v_strides = _rows16_args(v)
+    q_out = k_out = None
+    Hq, q_ptr, q_strides = 0, None, (0, 0, 0)
+    if q is not None:
+        Hq = q.shape[1]
+        q, q_ptr, q_strides = _rows16_args(q)
+        q_out = q.new_empty(B, Hq, S, D)
+    if want_k:
+        k_out = k.new_empty(B, Hkv, S, D)
+    lib = _lib.load()
+    with _on_device_of(k):
+        rc = lib.pbs_paged_append(
+            q_ptr, k_ptr, v_ptr, _ptr(cos), _ptr(sin), _ptr(q_out), _ptr(k_out), pages.k.data_ptr(), pages.v.data_ptr(), _ptr(pages.k_scale),
+            _ptr(pages.v_scale), page_table.data_ptr(), past_lens.data_ptr(), _ptr(new_lens), B, Hq, Hkv, S, D, n, max_pages, page_size, bits,
+            *q_strides, *k_strides, *v_strides, c_sb, c_ss, page_table.stride(0), _stream())
+    if rc:
+        _lib.check(rc, "pbs_paged_append")
+    return q_out, k_out
+
+
+def paged_read(pages, page_table, lens, max_len):
+    """The first ``lens[b]`` tokens of every sequence of a paged cache: (k, v), each (B, Hkv, max_len, 128) bf16, contiguous; rows from
+    ``lens[b]`` on are zeros, as are the tokens of pages that are not in the pool."""
+    B, Hkv = page_table.shape[0], pages.k.shape[1]
+    n, max_pages, page_size, bits = _check_paged(pages, page_table, B, Hkv, (lens,))
+    if max_len <= 0:
+        raise ValueError(f"max_len must be positive, got {max_len}")
+    k_out = torch.empty((B, Hkv, max_len, HEAD_DIM), dtype=torch.bfloat16, device=pages.k.device)
+    v_out = torch.empty_like(k_out)
+    lib = _lib.load()
+    with _on_device_of(k_out):
+        rc = lib.pbs_paged_read(pages.k.data_ptr(), pages.v.data_ptr(), _ptr(pages.k_scale), _ptr(pages.v_scale), page_table.data_ptr(),
+                                lens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), B, Hkv, max_len, HEAD_DIM, n, max_pages, page_size, bits,
+                                page_table.stride(0), _stream())
+    if rc:
+        _lib.check(rc, "pbs_paged_read")
+    return k_out, v_out
+
+
+def paged_attn(q, pages, page_table, past_lens, new_lens=None, softmax_scale=None, max_len=None):
+    """Attention of q (B, Hq, S, 128), the new tokens' queries, over a paged cache that holds their keys and values already
+    (``paged_append``): query i of sequence b sees its tokens 0 .. ``past_lens[b] + i``.  Returns (B, Hq, S, 128); rows from
+    ``new_lens[b]`` on (None: S) and rows that see no key are zeros.  ``max_len``: a length that no sequence exceeds, the new tokens
+    included, where the caller knows one (default: what the table has room for); it decides how the work is cut up, not the result's meaning."""
+    B, Hq, S, D = q.shape
+    Hkv = pages.k.shape[1]
+    assert D == HEAD_DIM and Hq % Hkv == 0
+    n, max_pages, page_size, bits = _check_paged(pages, page_table, B, Hkv, (past_lens, new_lens), q)
+    room = max_pages * page_size
+    max_len = room if max_len is None else min(max_len, room)
+    if softmax_scale is None:
+        softmax_scale = D ** -0.5
+    q, q_ptr, q_strides = _rows16_args(q)
+    out = q.new_empty(B, Hq, S, D)
+    lib = _lib.load()
+    ws_bytes = lib.pbs_paged_attn_workspace_bytes(B, Hq, Hkv, S, D, max_len)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _on_device_of(q):
+        rc = lib.pbs_paged_attn_fwd(
+            q_ptr, pages.k.data_ptr(), pages.v.data_ptr(), _ptr(pages.k_scale), _ptr(pages.v_scale), page_table.data_ptr(), past_lens.data_ptr(),
+            _ptr(new_lens), out.data_ptr(), B, Hq, Hkv, S, D, n, max_pages, page_size, bits, max_len, *q_strides, Hq * S * D, S * D, D,
+            page_table.stride(0), softmax_scale, _ptr(ws), ws_bytes, _stream())
+    if rc:
+        _lib.check(rc, "pbs_paged_attn_fwd")
+    return out
 
 
 def unpermute(o_perm, q_idx=None, out=None):

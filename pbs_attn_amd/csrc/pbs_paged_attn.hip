@@ -11,20 +11,33 @@
 
 namespace {
 
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+constexpr int WAVES = 4;
+constexpr int O_PITCH = PAGED_D + 4;
+constexpr int WORKERS = 512;   // workgroups of a launch that cuts sequences: two a compute unit
+constexpr int LEAST_STEPS = 2;   // steps (128 * NT keys) that a worker takes at least
+
+struct Header {   // of a worker: the piece of work that it began and left to the `more` workers after it
+  int unit, head, more, pad;
+};
+
 struct AttnArgs {
   PagedPool pool;
   const uint16_t* q;
   uint16_t* out;
   const int32_t* past;
   const int32_t* fresh;   // null: S
-  int B, Hq, Hkv, S, G;
+  Header* headers;        // one a worker; null: a workgroup takes a whole row tile of one head
+  float* parts;           // two slots a worker: the end of an earlier worker's piece, the beginning of the next one's
+  int B, Hq, Hkv, S, G, row_tiles;
   int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
   float scale_log2;   // softmax scale times log2(e)
 };
 
-constexpr int WAVES = 4;
-constexpr int ROWS = 16;
-constexpr int O_PITCH = PAGED_D + 4;
+template <int R>
+constexpr int slot_floats() { return R * 16 * (PAGED_D + 2); }
 
 __device__ __forceinline__ float max_over_groups(float v) {   // lanes l, l ^ 16, l ^ 32, l ^ 48
   TwoOf t = with_lane_xor<16>(__float_as_uint(v));
@@ -39,145 +52,504 @@ __device__ __forceinline__ float sum_over_groups(float v) {
   return __uint_as_float(t.a) + __uint_as_float(t.b);
 }
 
-// Lanes: n = lane % 16, g = lane / 16.  S^T = K Q^T by 16x16x32: operand row m of tile half a is token 2m + a, so that a lane ends up with
-// the logits of tokens 8g .. 8g + 7 for query row n, which are its share of P^T in O^T += V^T P^T: probabilities never change lanes.
+// a row tile of a sequence
+struct Unit {
+  int b, r0, past, fresh;
+  int keys;      // that its last token sees
+  int all_see;   // that its first token sees
+};
+template <int R>
+__device__ __forceinline__ Unit unit_of(const AttnArgs& a, int u) {
+  Unit t;
+  t.b = a.row_tiles == 1 ? u : u / a.row_tiles;
+  t.r0 = (u - t.b * a.row_tiles) * (R * 16);
+  t.past = min(max(a.past[t.b], 0), PAGED_MAX_TOKENS);
+  t.fresh = a.fresh ? min(max(a.fresh[t.b], 0), a.S) : a.S;
+  const int first = t.r0 / a.G, last = min(t.fresh - 1, (t.r0 + R * 16 - 1) / a.G);
+  t.keys = first < t.fresh ? min(t.past + last + 1, a.pool.max_pages << a.pool.page_shift) : 0;
+  t.all_see = t.past + first + 1;
+  return t;
+}
+__device__ __forceinline__ int steps_of(int keys, int step) { return max((keys + step - 1) / step, 1); }
+
+// What a lane holds of a tile of 32 tokens.  n = lane % 16, g = lane / 16.
 template <int BITS>
-__global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, head = blockIdx.y, r0 = blockIdx.x * ROWS;
-  const int past = min(max(a.past[b], 0), PAGED_MAX_TOKENS), fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
-  const int row = r0 + n, token = row / a.G, qh = head * a.G + row % a.G;
-  const bool valid = token < fresh;
-  __shared__ float o_lds[WAVES][ROWS][O_PITCH];
-  __shared__ float m_lds[WAVES][ROWS], l_lds[WAVES][ROWS];
+struct Tile;
+template <>
+struct Tile<16> {
+  u32x4 k[8], v[8];
+};
+template <>
+struct Tile<4> {
+  u32x4 k[2], v[2];
+  uint32_t ks;
+  u32x2 vs;
+};
+__device__ __forceinline__ void load_k(Tile<16>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* k = p.k + at * paged_tile_bytes<16>() + n * 512 + g * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t.k[h * 4 + c] = *(const u32x4*)(k + h * 256 + c * 64);
+}
+__device__ __forceinline__ void load_v(Tile<16>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* v = p.v + at * paged_tile_bytes<16>() + g * 2048 + n * 16;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) t.v[d] = *(const u32x4*)(v + d * 256);
+}
+__device__ __forceinline__ void load_k(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* k = p.k + at * paged_tile_bytes<4>() + n * 128 + g * 16;
+  t.k[0] = *(const u32x4*)k;
+  t.k[1] = *(const u32x4*)(k + 64);
+  t.ks = *(const uint16_t*)(p.ks + at * 128 + g * 32 + n * 2);
+}
+__device__ __forceinline__ void load_v(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* v = p.v + at * paged_tile_bytes<4>() + g * 512 + n * 16;
+  t.v[0] = *(const u32x4*)v;
+  t.v[1] = *(const u32x4*)(v + 256);
+  t.vs = *(const u32x2*)(p.vs + at * 128 + (n >> 2) * 32 + g * 8);
+}
 
-  const int seen = valid ? past + token + 1 : 0;                          // keys of this lane's row
-  const int last = min(fresh - 1, (r0 + ROWS - 1) / a.G);                 // the tile's last token
-  const int keys = min(r0 / a.G < fresh ? past + last + 1 : 0, a.pool.max_pages << a.pool.page_shift);
-  const int all_see = past + r0 / a.G + 1;                                // keys that every row sees
-
+// 16 query rows as the matrix instruction's right operand
+template <int BITS>
+struct Rows;
+template <>
+struct Rows<16> {
   bf16x8 q[4];
+  __device__ __forceinline__ void load(const uint16_t* row, int g) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u32x4 x = {};
+      if (row) x = *(const u32x4*)(row + c * 32 + g * 8);
+      q[c] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+};
+// For 4-bit keys the queries are the sum of two e4m3 numbers a channel: the matrix instruction then takes the keys as they lie in memory, with
+// their scales.  A bf16 value has 8 bits, e4m3 4: q = 2^e (hi + lo / 32) with hi = e4m3(q / 2^e) and lo the 4 bits that are left, exact down to 2^-21
+// of the row's largest channel (below it both halves are subnormal and lo is rounded).
+template <>
+struct Rows<4> {
+  i32x8 hi, lo;
+  int scale_hi, scale_lo;
+  __device__ __forceinline__ void load(const uint16_t* row, int g) {
+    u32x4 x[4] = {};   // channels 16 g .. 16 g + 15 and 64 + 16 g ..: 32 bytes of an 8-bit operand
+    if (row) {
+      x[0] = *(const u32x4*)(row + g * 16);
+      x[1] = *(const u32x4*)(row + g * 16 + 8);
+      x[2] = *(const u32x4*)(row + 64 + g * 16);
+      x[3] = *(const u32x4*)(row + 64 + g * 16 + 8);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(x[i][e] & 0x7fffu, (x[i][e] >> 16) & 0x7fffu));
+    TwoOf t = with_lane_xor<16>(top);
+    top = max(t.a, t.b);
+    t = with_lane_xor<32>(top);
+    top = max(t.a, t.b);
+    const int field = max((int)(top >> 7), 20);
+    const float up = __uint_as_float((uint32_t)(261 - field) << 23);   // the row's largest magnitude becomes 128 .. 256
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t a = x[w >> 1][(w & 1) * 2], b = x[w >> 1][(w & 1) * 2 + 1];
+      const float y0 = bf16_bits_to_f32(a & 0xffffu) * up, y1 = __uint_as_float(a & 0xffff0000u) * up;
+      const float y2 = bf16_bits_to_f32(b & 0xffffu) * up, y3 = __uint_as_float(b & 0xffff0000u) * up;
+      int h = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+      h = __builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, h, true);
+      int l = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 32.f, (y1 - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 32.f, 0, false);
+      l = __builtin_amdgcn_cvt_pk_fp8_f32((y2 - __builtin_amdgcn_cvt_f32_fp8(h, 2)) * 32.f, (y3 - __builtin_amdgcn_cvt_f32_fp8(h, 3)) * 32.f, l, true);
+      hi[w] = h;
+      lo[w] = l;
+    }
+    scale_hi = field >= 255 ? 255 : field - 7;    // (an infinity or NaN among the queries: NaN)
+    scale_lo = field >= 255 ? 255 : field - 12;
+  }
+};
+
+// S^T of one half (16 keys, operand row m = token 2 m + half) and 16 query rows
+__device__ __forceinline__ f32x4 logits(const Tile<16>& t, int half, const Rows<16>& r) {
+  f32x4 s = {};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[half * 4 + c]), r.q[c], s, 0, 0, 0);
+  return s;
+}
+template <int HALF>
+__device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
+  const i32x8 k = {(int)t.k[HALF][0], (int)t.k[HALF][1], (int)t.k[HALF][2], (int)t.k[HALF][3], 0, 0, 0, 0};
+  f32x4 s = {};
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 4, 0, HALF, (int)t.ks, 0, r.scale_hi);
+}
+__device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
+
+// V^T operands: v[d] holds eight tokens (8 g ..) of channel 16 d + n, of 4-bit pages of channel 8 n + d.  `held` of the eight are there.
+template <bool TAIL>
+__device__ __forceinline__ void values(const Tile<16>& t, int held, bf16x8 (&v)[8]) {
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    u32x4 x = t.v[d];
+    if (TAIL) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) x[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
+    }
+    v[d] = __builtin_bit_cast(bf16x8, x);
+  }
+}
+template <bool TAIL>
+__device__ __forceinline__ void values(const Tile<4>& t, int held, bf16x8 (&v)[8]) {
+  u32x4 x[8];   // token j: channels 8 n .. 8 n + 7
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t e = (t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu;
+    if (TAIL) e = j < held ? e : 0u;   // (codes are finite whatever the page held before)
+    x[j] = fp4_values(t.v[j >> 2][j & 3], __uint_as_float(e << 23));
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    u32x4 x = {};
-    if (valid) x = *(const u32x4*)(a.q + b * a.q_sb + qh * a.q_sh + (int64_t)token * a.q_ss + c * 32 + g * 8);
-    q[c] = __builtin_bit_cast(bf16x8, x);
+    u32x4 lo, hi;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      lo[w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x05040100u);
+      hi[w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x07060302u);
+    }
+    v[2 * c] = __builtin_bit_cast(bf16x8, lo);
+    v[2 * c + 1] = __builtin_bit_cast(bf16x8, hi);
   }
-  f32x4 o[8] = {};
-  float m = -FLT_MAX, l = 0.f;
-  for (int t = wave; t * PAGED_TILE < keys; t += WAVES) {
-    const int64_t at = paged_tile_index(a.pool, b, head, t);
-    if (at < 0) continue;
-    f32x4 st[2] = {};
+}
+template <int BITS>
+__device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? d * 16 + row : row * 8 + d; }
+
+// One wave's running softmax over its tiles.  S^T = K Q^T leaves a lane with the logits of tokens 8 g .. 8 g + 7 for query row n, which are
+// its share of P^T in O^T += V^T P^T: probabilities never change lanes.
+template <int BITS, int R, int NT>
+struct Softmax {
+  Rows<BITS> rows[R];
+  f32x4 o[R][8];
+  float m[R], l[R];
+  int seen[R];
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, const Unit& u, int head, int n, int g) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int r = 0; r < R; ++r) {
+      const int row = u.r0 + r * 16 + n, token = row / a.G;
+      const bool valid = token < u.fresh;
+      rows[r].load(valid ? a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss : nullptr, g);
+      seen[r] = valid ? u.past + token + 1 : 0;
+      m[r] = -FLT_MAX;
+      l[r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u32x4 k;
-        if (BITS == 16) {
-          k = *(const u32x4*)(a.pool.k + at * paged_tile_bytes<16>() + (2 * n + h) * 256 + c * 64 + g * 16);
-        } else {
-          const uint32_t w = *(const uint32_t*)(a.pool.k + at * paged_tile_bytes<4>() + (2 * n + h) * 64 + c * 16 + g * 4);
-          k = fp4_values(w, __uint_as_float((uint32_t)a.pool.ks[at * 128 + c * 32 + 2 * n + h] << 23));
-        }
-        st[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), q[c], st[h], 0, 0, 0);
-      }
+      for (int d = 0; d < 8; ++d) o[r][d] = (f32x4){};
     }
-    // st[h][i]: token 8g + 2i + h
-    float x[8];
+  }
+  // logits of the NT tiles; `k0`: the first one's first key, `keys`: how many there are, bit i of `gone`: tile i's page is not there
+  template <bool MASK>
+  __device__ __forceinline__ void weigh(const Tile<BITS> (&t)[NT], bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, float c, int g) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = st[j & 1][j >> 1] * a.scale_log2;
-    const int k0 = t * PAGED_TILE;
-    if (k0 + PAGED_TILE > all_see) {
+    for (int r = 0; r < R; ++r) {
+      float x[NT][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = k0 + 8 * g + j < seen ? x[j] : -INFINITY;
-    }
-    float top = x[0];
+      for (int i = 0; i < NT; ++i) {
+        const f32x4 s0 = logits(t[i], 0, rows[r]), s1 = logits(t[i], 1, rows[r]);
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-    const float m_new = fmaxf(m, max_over_groups(top));
-    const float scale = exp2f(m - m_new);
-    m = m_new;
-    l *= scale;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) o[d] *= scale;
-    bf16x8 p;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = exp2f(x[j] - m);
-      l += e;
-      p[j] = (__bf16)e;   // (weights of at most 1, half a step of 2^-8 off: they are summed as they are, and multiply bf16 values)
-    }
-    // tokens behind the keys hold whatever the page held before: not even times zero
-    const int held = keys - k0 - 8 * g;   // of this lane's eight
-    u32x4 v[8];
-    if (BITS == 16) {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        v[d] = *(const u32x4*)(a.pool.v + at * paged_tile_bytes<16>() + (g * PAGED_D + d * 16 + n) * 16);
-        if (k0 + PAGED_TILE > keys) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) v[d][w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
+        for (int j = 0; j < 8; ++j) {
+          x[i][j] = (j & 1) ? s1[j >> 1] : s0[j >> 1];
+          if (MASK) {
+            const int key = k0 + i * PAGED_TILE + 8 * g + j;
+            x[i][j] = key < min(seen[r], keys) && !(gone >> i & 1) ? x[i][j] : -INFINITY;
+          }
         }
       }
-    } else {
-      u32x4 x[8];   // token j: channels 8n .. 8n + 7
+      float top = x[0][0];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t w = *(const uint32_t*)(a.pool.v + at * paged_tile_bytes<4>() + ((2 * g + (j >> 2)) * 16 + n) * 16 + (j & 3) * 4);
-        const uint32_t e = a.pool.vs[at * 128 + (n >> 2) * 32 + 8 * g + j];
-        x[j] = fp4_values(w, __uint_as_float(e << 23));
-        if (j >= held) x[j] = (u32x4){};
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, x[i][j]);
+      const float m_new = fmaxf(m[r], max_over_groups(top) * c);
+      if (__any(m_new > m[r])) {
+        const float f = __builtin_amdgcn_exp2f(m[r] - m_new);
+        l[r] *= f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[r][d] *= f;
+        m[r] = m_new;
       }
+      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          v[2 * c][w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x05040100u);
-          v[2 * c + 1][w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x07060302u);
+        for (int j = 0; j < 8; ++j) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], c, -m[r]));
+          sum += e;
+          p[r][i][j] = (__bf16)e;   // (weights of at most 1, half a step of 2^-8 off: they are summed as they are, and multiply bf16 values)
         }
+      l[r] += sum;
     }
+  }
+  template <bool TAIL>
+  __device__ __forceinline__ void add(const Tile<BITS> (&t)[NT], const bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, int g) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v[d]), p, o[d], 0, 0, 0);
+    for (int i = 0; i < NT; ++i) {
+      bf16x8 v[8];
+      // tokens behind the keys hold whatever the page held before: not even times zero
+      values<TAIL>(t[i], gone >> i & 1 ? 0 : keys - k0 - i * PAGED_TILE - 8 * g, v);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d], p[r][i], o[r][d], 0, 0, 0);
+    }
+  }
+};
+
+// Steps `s0` .. `s0 + steps - 1` of a unit and head, 4 * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
+template <int BITS, int R, int NT>
+__device__ __forceinline__ void work(const AttnArgs& a, const Unit& u, int head, int s0, int steps, float* part,
+                                     float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  Softmax<BITS, R, NT> s;
+  s.begin(a, u, head, n, g);
+  const int tiles = (u.keys + PAGED_TILE - 1) / PAGED_TILE;
+  int t = (s0 * WAVES + wave) * NT;                             // this wave's first tile of the step
+  const int end = min((s0 + steps) * WAVES * NT, tiles);
+  Tile<BITS> tile[NT];
+  uint32_t gone = 0;
+  // pages are looked up a step ahead; a tile that is not there is read as the pool's first one, and not used
+  auto look_up = [&](int t, int64_t (&at)[NT]) __attribute__((always_inline)) {
+    uint32_t none = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      at[i] = t + i < tiles ? paged_tile_index(a.pool, u.b, head, t + i) : -1;
+      none |= (at[i] < 0 ? 1u : 0u) << i;
+      at[i] = max(at[i], (int64_t)0);
+    }
+    return none;
+  };
+  int64_t at[NT];
+  if (t < end) {
+    gone = look_up(t, at);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
+  }
+  while (t < end) {
+    const int next = t + WAVES * NT, k0 = t * PAGED_TILE;
+    const bool whole = k0 + NT * PAGED_TILE <= min(u.all_see, u.keys) && gone == 0;
+    uint32_t gone_next = 0;
+    if (next < end) gone_next = look_up(next, at);
+    bf16x8 p[R][NT];
+    if (whole) s.template weigh<false>(tile, p, k0, u.keys, gone, a.scale_log2, g);
+    else s.template weigh<true>(tile, p, k0, u.keys, gone, a.scale_log2, g);
+    if (next < end) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
+    }
+    if (whole) s.template add<false>(tile, p, k0, u.keys, gone, g);
+    else s.template add<true>(tile, p, k0, u.keys, gone, g);
+    if (next < end) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
+    }
+    gone = gone_next;
+    t = next;
   }
 
-  l = sum_over_groups(l);
-  if (g == 0) { m_lds[wave][n] = m; l_lds[wave][n] = l; }
-  __syncthreads();
-  float top = m_lds[0][n], sum = 0.f;
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m_lds[w][n]);
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) sum += l_lds[w][n] * exp2f(m_lds[w][n] - top);
-  // (rows without a token weigh the keys that every row sees: their sums are dropped here)
-  const float f = (sum == 0.f || !valid ? 0.f : 1.f / sum) * exp2f(m - top);
-#pragma unroll
-  for (int d = 0; d < 8; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // operand row 4g + i of tile d: channel 16 d + 4 g + i, of 4-bit pages channel 8 (4 g + i) + d
-      const int channel = BITS == 16 ? d * 16 + 4 * g + i : (4 * g + i) * 8 + d;
-      o_lds[wave][n][channel] = f == 0.f ? 0.f : o[d][i] * f;
+  for (int r = 0; r < R; ++r) {
+    const float l = sum_over_groups(s.l[r]);
+    if (r > 0) __syncthreads();   // (the rows before have been read)
+    if (g == 0) {
+      ml_lds[wave][n][0] = s.m[r];
+      ml_lds[wave][n][1] = l;
     }
-  __syncthreads();
-  // 16 lanes a row, 8 channels a lane
-  const int rr = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8;
-  const int tok = (r0 + rr) / a.G, h = head * a.G + (r0 + rr) % a.G;
-  if (tok >= a.S) return;
-  u32x4 y;
+    __syncthreads();
+    float top = ml_lds[0][n][0];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f32x2 s = {};
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, ml_lds[w][n][0]);
+    const float f = __builtin_amdgcn_exp2f(s.m[r] - top);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += (f32x2){o_lds[w][rr][c + 2 * e], o_lds[w][rr][c + 2 * e + 1]};
-    y[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(s, bf16x2));
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o_lds[wave][n][channel_of<BITS>(d, 4 * g + i)] = f == 0.f ? 0.f : s.o[r][d][i] * f;
+    __syncthreads();
+    // 16 lanes a row, 8 channels a lane
+    const int rr = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
+    float y[8], row_top = ml_lds[0][rr][0], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) row_top = fmaxf(row_top, ml_lds[w][rr][0]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += ml_lds[w][rr][1] * __builtin_amdgcn_exp2f(ml_lds[w][rr][0] - row_top);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) y[e] += o_lds[w][rr][c + e];
+    }
+    if (part) {
+      float* dst = part + (r * 16 + rr) * PAGED_D + c;
+      *(f32x4*)dst = (f32x4){y[0], y[1], y[2], y[3]};
+      *(f32x4*)(dst + 4) = (f32x4){y[4], y[5], y[6], y[7]};
+      if (c == 0) *(f32x2*)(part + R * 16 * PAGED_D + (r * 16 + rr) * 2) = (f32x2){row_top, sum};
+    } else if (token < a.S) {
+      // (rows without a token weigh the keys that every row sees: their sums are dropped here)
+      const float scale = sum == 0.f || token >= u.fresh ? 0.f : 1.f / sum;
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = scale == 0.f ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){y[2 * e] * scale, y[2 * e + 1] * scale}, bf16x2));
+      *(u32x4*)(a.out + u.b * a.o_sb + (head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + c) = w;
+    }
   }
-  *(u32x4*)(a.out + b * a.o_sb + h * a.o_sh + (int64_t)tok * a.o_ss + c) = y;
+  __syncthreads();
+}
+
+// Without headers: a workgroup per row tile and head (blockIdx: head, row tile of a sequence).  With them: the steps of all row tiles and heads in
+// one line (sequence, row tile, head, step), cut into equal pieces, one a workgroup, so that sequences of any lengths fill the chip.
+template <int BITS, int R, int NT>
+__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
+  constexpr int STEP = WAVES * NT * PAGED_TILE;
+  __shared__ float o_lds[WAVES][16][O_PITCH];
+  __shared__ float ml_lds[WAVES][16][2];
+  __shared__ int64_t wave_sums[WAVES];
+  __shared__ int first_unit;
+  __shared__ int64_t first_left;
+  int index = blockIdx.y, head = blockIdx.x, step = 0;
+  int64_t share = INT32_MAX, todo = 0;
+  if (a.headers) {
+    // where this worker's piece begins: running sums over the row tiles, a stretch of them a thread
+    const int units = a.B * a.row_tiles, stretch = (units + 255) / 256, from = min((int)threadIdx.x * stretch, units), to = min(from + stretch, units);
+    int64_t mine = 0;
+    for (int i = from; i < to; ++i) mine += (int64_t)a.Hkv * steps_of(unit_of<R>(a, i).keys, STEP);
+    int64_t before = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t other = __shfl_up(before, d, 64);
+      if ((threadIdx.x & 63) >= d) before += other;
+    }
+    if ((threadIdx.x & 63) == 63) wave_sums[threadIdx.x >> 6] = before;
+    before -= mine;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) before += wave_sums[w];
+      total += wave_sums[w];
+    }
+    share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)LEAST_STEPS);
+    const int64_t start = share * blockIdx.x;
+    if (start >= total) {
+      if (threadIdx.x == 0) a.headers[blockIdx.x].more = 0;
+      return;
+    }
+    if (start >= before && start < before + mine) {
+      int64_t left = start - before;
+      for (int i = from;; ++i) {
+        const int64_t cost = (int64_t)a.Hkv * steps_of(unit_of<R>(a, i).keys, STEP);
+        if (left < cost) {
+          first_unit = i;
+          first_left = left;
+          break;
+        }
+        left -= cost;
+      }
+    }
+    __syncthreads();
+    index = __builtin_amdgcn_readfirstlane(first_unit);
+    todo = min(share, total - start);
+  }
+  Unit u = unit_of<R>(a, index);
+  int steps = steps_of(u.keys, STEP);
+  if (a.headers) {
+    head = __builtin_amdgcn_readfirstlane((int)(first_left / steps));
+    step = __builtin_amdgcn_readfirstlane((int)(first_left % steps));
+  } else {
+    todo = steps;
+  }
+  int more = 0;
+  while (true) {
+    const int n = (int)min((int64_t)(steps - step), todo);
+    todo -= n;
+    float* part = nullptr;
+    if (step > 0 || n < steps) part = a.parts + ((int64_t)blockIdx.x * 2 + (step == 0)) * slot_floats<R>();
+    if (step == 0 && n < steps) more = (int)((steps - n + share - 1) / share);
+    work<BITS, R, NT>(a, u, head, step, n, part, o_lds, ml_lds);
+    if (todo == 0) break;
+    step = 0;
+    if (++head == a.Hkv) {
+      head = 0;
+      u = unit_of<R>(a, ++index);
+      steps = steps_of(u.keys, STEP);
+    }
+  }
+  if (a.headers && threadIdx.x == 0) a.headers[blockIdx.x] = {index, head, more, 0};
+}
+
+// Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it, in order.  A wave a row.
+template <int R>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  const Header h = a.headers[blockIdx.x];
+  if (h.more == 0) return;
+  const Unit u = unit_of<R>(a, h.unit);
+  const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), row = u.r0 + rr, token = row / a.G;
+  if (token >= a.S) return;
+  const float* first = a.parts + ((int64_t)blockIdx.x * 2 + 1) * slot_floats<R>();
+  // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
+  auto part = [&](int i) { return first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot_floats<R>()); };
+  float top = -FLT_MAX;
+  for (int i = lane; i <= h.more; i += 64) top = fmaxf(top, part(i)[R * 16 * PAGED_D + rr * 2]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  float sum = 0.f;
+  f32x2 y = {};
+#pragma unroll 4
+  for (int i = 0; i <= h.more; ++i) {
+    const float* p = part(i);
+    const f32x2 ml = *(const f32x2*)(p + R * 16 * PAGED_D + rr * 2), x = *(const f32x2*)(p + rr * PAGED_D + lane * 2);
+    const float f = __builtin_amdgcn_exp2f(ml.x - top);
+    sum += ml.y * f;
+    if (f != 0.f) y += x * f;
+  }
+  const float scale = sum == 0.f || token >= u.fresh ? 0.f : 1.f / sum;
+  const uint32_t w = scale == 0.f ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){y.x * scale, y.y * scale}, bf16x2));
+  *(uint32_t*)(a.out + u.b * a.o_sb + (h.head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + lane * 2) = w;
+}
+
+struct Plan {
+  int rows;   // 16-row tiles of a workgroup
+  bool cut;
+  size_t bytes;
+};
+Plan plan_of(int Hq, int Hkv, int S, int max_len) {
+  Plan p;
+  const int64_t rows = (int64_t)S * (Hq / Hkv);
+  p.rows = rows <= 16 ? 1 : 2;
+  p.cut = max_len > 512;
+  const size_t slot = (size_t)p.rows * 16 * (PAGED_D + 2) * sizeof(float);
+  p.bytes = p.cut ? WORKERS * (sizeof(Header) + 2 * slot) : 0;
+  return p;
+}
+
+template <int BITS, int R, int NT>
+void launch(const AttnArgs& a, bool cut, hipStream_t stream) {
+  if (!cut) {
+    hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(a.Hkv, a.B * a.row_tiles), dim3(256), 0, stream, a);
+    return;
+  }
+  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(WORKERS), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(join_kernel<R>, dim3(WORKERS, R * 16 / WAVES), dim3(256), 0, stream, a);
+}
+template <int BITS, int NT>
+void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t stream) {
+  if (p.rows == 1) launch<BITS, 1, NT>(a, p.cut, stream);
+  else launch<BITS, 2, NT>(a, p.cut, stream);
 }
 
 }  // namespace
 
-extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len) { return 0; }
+extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || S <= 0 || Hq < Hkv || max_len <= 0) return 0;
+  return plan_of(Hq, Hkv, S, max_len).bytes;
+}
 
 extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                                   const int32_t* page_table, const int32_t* past_lens, const int32_t* new_lens, void* out, int B, int Hq, int Hkv,
@@ -191,15 +563,22 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   PBS_REQUIRE(q && out && past_lens, "pbs_paged_attn_fwd: null tensor pointer");
   PBS_REQUIRE(S > 0 && S <= (1 << 26) && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0, "pbs_paged_attn_fwd: bad shape");
   PBS_REQUIRE((int64_t)S * (Hq / Hkv) <= (1 << 26), "pbs_paged_attn_fwd: too many query rows");
+  PBS_REQUIRE(max_len > 0, "pbs_paged_attn_fwd: max_len must be positive");
   PBS_REQUIRE(softmax_scale > 0.f && softmax_scale <= FLT_MAX, "pbs_paged_attn_fwd: softmax_scale must be positive and finite");
   PBS_REQUIRE(((q_sb | q_sh | q_ss | o_sb | o_sh | o_ss) % 8) == 0, "pbs_paged_attn_fwd: strides must keep rows 16-byte aligned");
   PBS_REQUIRE((((uintptr_t)q | (uintptr_t)out) % 16) == 0, "pbs_paged_attn_fwd: pointers must be 16-byte aligned");
+  const Plan p = plan_of(Hq, Hkv, S, max_len);
+  PBS_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace % 256) == 0 && workspace_bytes >= p.bytes),
+              "pbs_paged_attn_fwd: workspace of %zu bytes, 256-byte aligned, needed", p.bytes);
   a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.past = past_lens; a.fresh = new_lens;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.S = S; a.G = Hq / Hkv;
   a.q_sb = q_sb; a.q_sh = q_sh; a.q_ss = q_ss; a.o_sb = o_sb; a.o_sh = o_sh; a.o_ss = o_ss;
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
-  const dim3 grid((S * a.G + ROWS - 1) / ROWS, Hkv, B);
-  if (kv_bits == 16) hipLaunchKernelGGL(attn_kernel<16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(attn_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  a.row_tiles = (S * a.G + p.rows * 16 - 1) / (p.rows * 16);
+  PBS_REQUIRE((int64_t)B * a.row_tiles <= (p.cut ? INT32_MAX : 65535), "pbs_paged_attn_fwd: too many query rows");
+  a.headers = p.cut ? (Header*)workspace : nullptr;
+  a.parts = p.cut ? (float*)((char*)workspace + WORKERS * sizeof(Header)) : nullptr;
+  if (kv_bits == 16) launch_rows<16, 1>(a, p, (hipStream_t)stream);
+  else launch_rows<4, 2>(a, p, (hipStream_t)stream);
   return pbs_check_launch("pbs_paged_attn_fwd");
 }

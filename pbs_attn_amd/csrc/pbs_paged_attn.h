@@ -1,0 +1,170 @@
+// Attention over a paged cache: what its kernels share.  Arguments, the row tiles of a sequence, and how the work is cut.
+#pragma once
+#include "pbs_paged.h"
+#include "pbs_wave.h"
+#include <float.h>
+
+constexpr int PAGED_WAVES = 4;       // of a workgroup
+constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences: two a compute unit
+constexpr int PAGED_LEAST_STEPS = 2;   // steps that a worker takes at least
+
+struct PagedHeader {   // of a worker: the piece of work that it began and left to the `more` workers after it
+  int unit, head, more, pad;
+};
+
+struct PagedAttnArgs {
+  PagedPool pool;
+  const uint16_t* q;
+  uint16_t* out;
+  const int32_t* past;
+  const int32_t* fresh;   // null: S
+  PagedHeader* headers;   // one a worker; null: a workgroup takes a whole row tile of one head
+  float* parts;           // two slots a worker: the end of an earlier worker's piece, the beginning of the next one's
+  int B, Hq, Hkv, S, G, row_tiles;
+  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
+  float scale_log2;   // softmax scale times log2(e)
+};
+
+// a slot: rows of 128 sums, then each row's largest exponent and sum of weights
+constexpr int paged_slot_floats(int rows) { return rows * (PAGED_D + 2); }
+
+__device__ __forceinline__ float max_over_groups(float v) {   // lanes l, l ^ 16, l ^ 32, l ^ 48
+  TwoOf t = with_lane_xor<16>(__float_as_uint(v));
+  v = fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
+  t = with_lane_xor<32>(__float_as_uint(v));
+  return fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+  TwoOf t = with_lane_xor<16>(__float_as_uint(v));
+  v = __uint_as_float(t.a) + __uint_as_float(t.b);
+  t = with_lane_xor<32>(__float_as_uint(v));
+  return __uint_as_float(t.a) + __uint_as_float(t.b);
+}
+
+// a sequence, and one of its row tiles
+struct PagedSeq {
+  int b, past, fresh;
+  int steps;         // of a row tile with tokens (the last one's: tiles before it see fewer keys, and idle for a while)
+  int64_t a_head;    // steps of one head: row tiles without tokens take one, in which their rows are cleared
+  int tiles;         // row tiles with tokens
+};
+template <int ROWS, int STEP>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b) {
+  PagedSeq s;
+  s.b = b;
+  s.past = min(max(a.past[b], 0), PAGED_MAX_TOKENS);
+  s.fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
+  s.tiles = (s.fresh * a.G + ROWS - 1) / ROWS;
+  s.steps = max((min(s.past + s.fresh, a.pool.max_pages << a.pool.page_shift) + STEP - 1) / STEP, 1);
+  s.a_head = (int64_t)s.tiles * s.steps + (a.row_tiles - s.tiles);
+  return s;
+}
+struct PagedUnit {
+  int b, r0, past, fresh;
+  int keys;      // that its last token sees
+  int all_see;   // that its first token sees
+};
+template <int ROWS>
+__device__ __forceinline__ PagedUnit paged_unit(const PagedAttnArgs& a, int b, int past, int fresh, int tile) {
+  PagedUnit t;
+  t.b = b; t.past = past; t.fresh = fresh;
+  t.r0 = tile * ROWS;
+  const int first = t.r0 / a.G, last = min(fresh - 1, (t.r0 + ROWS - 1) / a.G);
+  t.keys = first < fresh ? min(past + last + 1, a.pool.max_pages << a.pool.page_shift) : 0;
+  t.all_see = past + first + 1;
+  return t;
+}
+
+// Where a workgroup begins, and how many steps are its.  The steps of all sequences lie in one line (sequence, head, row tile, step), cut
+// into equal shares, one a worker, so that sequences of any lengths fill the chip.
+struct PagedShare {
+  int worker, b, head, tile, step;
+  int64_t todo, share;
+};
+struct PagedShareLds {
+  int64_t wave_sums[PAGED_WAVES], left;
+  int b;
+};
+template <int ROWS, int STEP>
+__device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int workers, PagedShare* out) {
+  const int tid = threadIdx.x, stretch = (a.B + 255) / 256, from = min(tid * stretch, a.B), to = min(from + stretch, a.B);
+  int64_t mine = 0;
+  for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+  int64_t before = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t other = __shfl_up(before, d, 64);
+    if ((tid & 63) >= d) before += other;
+  }
+  if ((tid & 63) == 63) lds.wave_sums[tid >> 6] = before;
+  before -= mine;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < PAGED_WAVES; ++w) {
+    if (w < (tid >> 6)) before += lds.wave_sums[w];
+    total += lds.wave_sums[w];
+  }
+  out->worker = worker;
+  out->share = max((total + workers - 1) / workers, (int64_t)PAGED_LEAST_STEPS);
+  const int64_t start = out->share * worker;
+  out->todo = min(out->share, total - start);
+  if (start >= total) return false;
+  if (start >= before && start < before + mine) {
+    int64_t left = start - before;
+    for (int i = from;; ++i) {
+      const int64_t cost = a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+      if (left < cost) {
+        lds.b = i;
+        lds.left = left;
+        break;
+      }
+      left -= cost;
+    }
+  }
+  __syncthreads();
+  const PagedSeq s = paged_seq<ROWS, STEP>(a, __builtin_amdgcn_readfirstlane(lds.b));
+  const int64_t head = lds.left / s.a_head, left = lds.left - head * s.a_head, full = (int64_t)s.tiles * s.steps;
+  out->b = s.b;
+  out->head = __builtin_amdgcn_readfirstlane((int)head);
+  out->tile = __builtin_amdgcn_readfirstlane((int)(left < full ? left / s.steps : s.tiles + (left - full)));
+  out->step = __builtin_amdgcn_readfirstlane((int)(left < full ? left % s.steps : 0));
+  return true;
+}
+
+// A workgroup's way through its share, or through the one row tile and head that are its without headers: work(unit, head, first step,
+// steps, part), part null where the steps are all that the row tile has.
+template <int ROWS, int STEP, class Work>
+__device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int tile, Work&& work) {
+  PagedShare at;
+  at.worker = worker; at.b = tile / a.row_tiles; at.head = blockIdx.x; at.tile = tile - at.b * a.row_tiles; at.step = 0;
+  at.share = at.todo = INT32_MAX;
+  if (a.headers && !paged_share<ROWS, STEP>(a, lds, worker, gridDim.x, &at)) {
+    if (threadIdx.x == 0) a.headers[worker].more = 0;
+    return;
+  }
+  int more = 0;
+  PagedSeq s = paged_seq<ROWS, STEP>(a, at.b);
+  while (true) {
+    const int steps = at.tile < s.tiles ? s.steps : 1, n = (int)min((int64_t)(steps - at.step), at.todo);
+    at.todo -= n;
+    float* part = nullptr;
+    if (n < steps) part = a.parts + ((int64_t)worker * 2 + (at.step == 0)) * paged_slot_floats(ROWS);
+    if (at.step == 0 && n < steps) more = (int)((steps - n + at.share - 1) / at.share);
+    work(paged_unit<ROWS>(a, s.b, s.past, s.fresh, at.tile), at.head, at.step, n, part);
+    if (!a.headers) return;
+    if (at.todo == 0) break;
+    at.step = 0;
+    if (++at.tile == a.row_tiles) {
+      at.tile = 0;
+      if (++at.head == a.Hkv) {
+        at.head = 0;
+        s = paged_seq<ROWS, STEP>(a, s.b + 1);
+      }
+    }
+  }
+  if (threadIdx.x == 0) a.headers[worker] = {s.b * a.row_tiles + at.tile, at.head, more, 0};
+}
+
+// many rows a row tile (csrc/pbs_paged_rows.hip)
+int paged_attn_rows(const PagedAttnArgs& a, int kv_bits, int rows, hipStream_t stream);

@@ -3,10 +3,8 @@
 // For query i of a sequence with `past` tokens before the call: o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q k_j - m), over the keys
 // j <= past + i, m the largest exponent so far (one pass: sums are rescaled where it grows).  All query heads of a KV head and several
 // tokens share a tile's rows, row r = (token r / G, head r % G of the group), so a key is read once for all of them.
-#include "pbs_paged.h"
-#include "pbs_wave.h"
+#include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
-#include <float.h>
 #include <math.h>
 
 namespace {
@@ -14,63 +12,8 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
-constexpr int WAVES = 4;
+constexpr int WAVES = PAGED_WAVES;
 constexpr int O_PITCH = PAGED_D + 4;
-constexpr int WORKERS = 512;   // workgroups of a launch that cuts sequences: two a compute unit
-constexpr int LEAST_STEPS = 2;   // steps (128 * NT keys) that a worker takes at least
-
-struct Header {   // of a worker: the piece of work that it began and left to the `more` workers after it
-  int unit, head, more, pad;
-};
-
-struct AttnArgs {
-  PagedPool pool;
-  const uint16_t* q;
-  uint16_t* out;
-  const int32_t* past;
-  const int32_t* fresh;   // null: S
-  Header* headers;        // one a worker; null: a workgroup takes a whole row tile of one head
-  float* parts;           // two slots a worker: the end of an earlier worker's piece, the beginning of the next one's
-  int B, Hq, Hkv, S, G, row_tiles;
-  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
-  float scale_log2;   // softmax scale times log2(e)
-};
-
-template <int R>
-constexpr int slot_floats() { return R * 16 * (PAGED_D + 2); }
-
-__device__ __forceinline__ float max_over_groups(float v) {   // lanes l, l ^ 16, l ^ 32, l ^ 48
-  TwoOf t = with_lane_xor<16>(__float_as_uint(v));
-  v = fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
-  t = with_lane_xor<32>(__float_as_uint(v));
-  return fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
-}
-__device__ __forceinline__ float sum_over_groups(float v) {
-  TwoOf t = with_lane_xor<16>(__float_as_uint(v));
-  v = __uint_as_float(t.a) + __uint_as_float(t.b);
-  t = with_lane_xor<32>(__float_as_uint(v));
-  return __uint_as_float(t.a) + __uint_as_float(t.b);
-}
-
-// a row tile of a sequence
-struct Unit {
-  int b, r0, past, fresh;
-  int keys;      // that its last token sees
-  int all_see;   // that its first token sees
-};
-template <int R>
-__device__ __forceinline__ Unit unit_of(const AttnArgs& a, int u) {
-  Unit t;
-  t.b = a.row_tiles == 1 ? u : u / a.row_tiles;
-  t.r0 = (u - t.b * a.row_tiles) * (R * 16);
-  t.past = min(max(a.past[t.b], 0), PAGED_MAX_TOKENS);
-  t.fresh = a.fresh ? min(max(a.fresh[t.b], 0), a.S) : a.S;
-  const int first = t.r0 / a.G, last = min(t.fresh - 1, (t.r0 + R * 16 - 1) / a.G);
-  t.keys = first < t.fresh ? min(t.past + last + 1, a.pool.max_pages << a.pool.page_shift) : 0;
-  t.all_see = t.past + first + 1;
-  return t;
-}
-__device__ __forceinline__ int steps_of(int keys, int step) { return max((keys + step - 1) / step, 1); }
 
 // What a lane holds of a tile of 32 tokens.  n = lane % 16, g = lane / 16.
 template <int BITS>
@@ -230,7 +173,7 @@ struct Softmax {
   float m[R], l[R];
   int seen[R];
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, const Unit& u, int head, int n, int g) {
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedUnit& u, int head, int n, int g) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = u.r0 + r * 16 + n, token = row / a.G;
@@ -303,7 +246,7 @@ struct Softmax {
 
 // Steps `s0` .. `s0 + steps - 1` of a unit and head, 4 * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
 template <int BITS, int R, int NT>
-__device__ __forceinline__ void work(const AttnArgs& a, const Unit& u, int head, int s0, int steps, float* part,
+__device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part,
                                      float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   Softmax<BITS, R, NT> s;
@@ -403,100 +346,28 @@ __device__ __forceinline__ void work(const AttnArgs& a, const Unit& u, int head,
   __syncthreads();
 }
 
-// Without headers: a workgroup per row tile and head (blockIdx: head, row tile of a sequence).  With them: the steps of all row tiles and heads in
-// one line (sequence, row tile, head, step), cut into equal pieces, one a workgroup, so that sequences of any lengths fill the chip.
 template <int BITS, int R, int NT>
-__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
-  constexpr int STEP = WAVES * NT * PAGED_TILE;
+__global__ __launch_bounds__(256, 2) void attn_kernel(PagedAttnArgs a) {
   __shared__ float o_lds[WAVES][16][O_PITCH];
   __shared__ float ml_lds[WAVES][16][2];
-  __shared__ int64_t wave_sums[WAVES];
-  __shared__ int first_unit;
-  __shared__ int64_t first_left;
-  int index = blockIdx.y, head = blockIdx.x, step = 0;
-  int64_t share = INT32_MAX, todo = 0;
-  if (a.headers) {
-    // where this worker's piece begins: running sums over the row tiles, a stretch of them a thread
-    const int units = a.B * a.row_tiles, stretch = (units + 255) / 256, from = min((int)threadIdx.x * stretch, units), to = min(from + stretch, units);
-    int64_t mine = 0;
-    for (int i = from; i < to; ++i) mine += (int64_t)a.Hkv * steps_of(unit_of<R>(a, i).keys, STEP);
-    int64_t before = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t other = __shfl_up(before, d, 64);
-      if ((threadIdx.x & 63) >= d) before += other;
-    }
-    if ((threadIdx.x & 63) == 63) wave_sums[threadIdx.x >> 6] = before;
-    before -= mine;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < (int)(threadIdx.x >> 6)) before += wave_sums[w];
-      total += wave_sums[w];
-    }
-    share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)LEAST_STEPS);
-    const int64_t start = share * blockIdx.x;
-    if (start >= total) {
-      if (threadIdx.x == 0) a.headers[blockIdx.x].more = 0;
-      return;
-    }
-    if (start >= before && start < before + mine) {
-      int64_t left = start - before;
-      for (int i = from;; ++i) {
-        const int64_t cost = (int64_t)a.Hkv * steps_of(unit_of<R>(a, i).keys, STEP);
-        if (left < cost) {
-          first_unit = i;
-          first_left = left;
-          break;
-        }
-        left -= cost;
-      }
-    }
-    __syncthreads();
-    index = __builtin_amdgcn_readfirstlane(first_unit);
-    todo = min(share, total - start);
-  }
-  Unit u = unit_of<R>(a, index);
-  int steps = steps_of(u.keys, STEP);
-  if (a.headers) {
-    head = __builtin_amdgcn_readfirstlane((int)(first_left / steps));
-    step = __builtin_amdgcn_readfirstlane((int)(first_left % steps));
-  } else {
-    todo = steps;
-  }
-  int more = 0;
-  while (true) {
-    const int n = (int)min((int64_t)(steps - step), todo);
-    todo -= n;
-    float* part = nullptr;
-    if (step > 0 || n < steps) part = a.parts + ((int64_t)blockIdx.x * 2 + (step == 0)) * slot_floats<R>();
-    if (step == 0 && n < steps) more = (int)((steps - n + share - 1) / share);
-    work<BITS, R, NT>(a, u, head, step, n, part, o_lds, ml_lds);
-    if (todo == 0) break;
-    step = 0;
-    if (++head == a.Hkv) {
-      head = 0;
-      u = unit_of<R>(a, ++index);
-      steps = steps_of(u.keys, STEP);
-    }
-  }
-  if (a.headers && threadIdx.x == 0) a.headers[blockIdx.x] = {index, head, more, 0};
+  __shared__ PagedShareLds share_lds;
+  paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, blockIdx.y, [&](const PagedUnit& u, int head, int step, int steps, float* part)
+                                            __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds); });
 }
 
 // Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it, in order.  A wave a row.
-template <int R>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
-  const Header h = a.headers[blockIdx.x];
+__global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
+  const PagedHeader h = a.headers[blockIdx.x];
   if (h.more == 0) return;
-  const Unit u = unit_of<R>(a, h.unit);
-  const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), row = u.r0 + rr, token = row / a.G;
+  const int b = h.unit / a.row_tiles, fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
+  const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), row = (h.unit - b * a.row_tiles) * rows + rr, token = row / a.G;
   if (token >= a.S) return;
-  const float* first = a.parts + ((int64_t)blockIdx.x * 2 + 1) * slot_floats<R>();
+  const int slot = paged_slot_floats(rows);
+  const float* first = a.parts + ((int64_t)blockIdx.x * 2 + 1) * slot;
   // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
-  auto part = [&](int i) { return first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot_floats<R>()); };
+  auto part = [&](int i) { return first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot); };
   float top = -FLT_MAX;
-  for (int i = lane; i <= h.more; i += 64) top = fmaxf(top, part(i)[R * 16 * PAGED_D + rr * 2]);
+  for (int i = lane; i <= h.more; i += 64) top = fmaxf(top, part(i)[rows * PAGED_D + rr * 2]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
   float sum = 0.f;
@@ -504,51 +375,42 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 #pragma unroll 4
   for (int i = 0; i <= h.more; ++i) {
     const float* p = part(i);
-    const f32x2 ml = *(const f32x2*)(p + R * 16 * PAGED_D + rr * 2), x = *(const f32x2*)(p + rr * PAGED_D + lane * 2);
+    const f32x2 ml = *(const f32x2*)(p + rows * PAGED_D + rr * 2), x = *(const f32x2*)(p + rr * PAGED_D + lane * 2);
     const float f = __builtin_amdgcn_exp2f(ml.x - top);
     sum += ml.y * f;
     if (f != 0.f) y += x * f;
   }
-  const float scale = sum == 0.f || token >= u.fresh ? 0.f : 1.f / sum;
+  const float scale = sum == 0.f || token >= fresh ? 0.f : 1.f / sum;
   const uint32_t w = scale == 0.f ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){y.x * scale, y.y * scale}, bf16x2));
-  *(uint32_t*)(a.out + u.b * a.o_sb + (h.head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + lane * 2) = w;
+  *(uint32_t*)(a.out + b * a.o_sb + (h.head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + lane * 2) = w;
 }
 
 struct Plan {
-  int rows;   // 16-row tiles of a workgroup
+  int rows;   // of a row tile
   bool cut;
   size_t bytes;
 };
-Plan plan_of(int Hq, int Hkv, int S, int max_len) {
+Plan plan_of(int B, int Hq, int Hkv, int S, int max_len) {
   Plan p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.rows = rows <= 16 ? 1 : 2;
-  p.cut = max_len > 512;
-  const size_t slot = (size_t)p.rows * 16 * (PAGED_D + 2) * sizeof(float);
-  p.bytes = p.cut ? WORKERS * (sizeof(Header) + 2 * slot) : 0;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const int64_t units = B * ((rows + p.rows - 1) / p.rows);
+  p.cut = max_len > 512 && (p.rows <= 32 || units * Hkv < 4 * PAGED_WORKERS);
+  if (units > 65535) p.cut = true;   // (a grid's second index)
+  p.bytes = p.cut ? PAGED_WORKERS * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows)) : 0;
   return p;
 }
 
 template <int BITS, int R, int NT>
-void launch(const AttnArgs& a, bool cut, hipStream_t stream) {
-  if (!cut) {
-    hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(a.Hkv, a.B * a.row_tiles), dim3(256), 0, stream, a);
-    return;
-  }
-  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(WORKERS), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL(join_kernel<R>, dim3(WORKERS, R * 16 / WAVES), dim3(256), 0, stream, a);
-}
-template <int BITS, int NT>
-void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t stream) {
-  if (p.rows == 1) launch<BITS, 1, NT>(a, p.cut, stream);
-  else launch<BITS, 2, NT>(a, p.cut, stream);
+void launch(const PagedAttnArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), a.headers ? dim3(PAGED_WORKERS) : dim3(a.Hkv, a.B * a.row_tiles), dim3(256), 0, stream, a);
 }
 
 }  // namespace
 
 extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || S <= 0 || Hq < Hkv || max_len <= 0) return 0;
-  return plan_of(Hq, Hkv, S, max_len).bytes;
+  return plan_of(B, Hq, Hkv, S, max_len).bytes;
 }
 
 extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
@@ -556,7 +418,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
                                   int S, int head_dim, int num_pages, int max_pages, int page_size, int kv_bits, int max_len, int64_t q_sb,
                                   int64_t q_sh, int64_t q_ss, int64_t o_sb, int64_t o_sh, int64_t o_ss, int64_t table_sb, float softmax_scale,
                                   void* workspace, size_t workspace_bytes, void* stream) {
-  AttnArgs a;
+  PagedAttnArgs a;
   if (const int rc = paged_pool(&a.pool, "pbs_paged_attn_fwd", k_pages, v_pages, k_scale, v_scale, page_table, table_sb, B, Hkv, head_dim, num_pages,
                                 max_pages, page_size, kv_bits))
     return rc;
@@ -567,18 +429,27 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   PBS_REQUIRE(softmax_scale > 0.f && softmax_scale <= FLT_MAX, "pbs_paged_attn_fwd: softmax_scale must be positive and finite");
   PBS_REQUIRE(((q_sb | q_sh | q_ss | o_sb | o_sh | o_ss) % 8) == 0, "pbs_paged_attn_fwd: strides must keep rows 16-byte aligned");
   PBS_REQUIRE((((uintptr_t)q | (uintptr_t)out) % 16) == 0, "pbs_paged_attn_fwd: pointers must be 16-byte aligned");
-  const Plan p = plan_of(Hq, Hkv, S, max_len);
+  const Plan p = plan_of(B, Hq, Hkv, S, max_len);
   PBS_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace % 256) == 0 && workspace_bytes >= p.bytes),
               "pbs_paged_attn_fwd: workspace of %zu bytes, 256-byte aligned, needed", p.bytes);
   a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.past = past_lens; a.fresh = new_lens;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.S = S; a.G = Hq / Hkv;
   a.q_sb = q_sb; a.q_sh = q_sh; a.q_ss = q_ss; a.o_sb = o_sb; a.o_sh = o_sh; a.o_ss = o_ss;
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
-  a.row_tiles = (S * a.G + p.rows * 16 - 1) / (p.rows * 16);
-  PBS_REQUIRE((int64_t)B * a.row_tiles <= (p.cut ? INT32_MAX : 65535), "pbs_paged_attn_fwd: too many query rows");
-  a.headers = p.cut ? (Header*)workspace : nullptr;
-  a.parts = p.cut ? (float*)((char*)workspace + WORKERS * sizeof(Header)) : nullptr;
-  if (kv_bits == 16) launch_rows<16, 1>(a, p, (hipStream_t)stream);
-  else launch_rows<4, 2>(a, p, (hipStream_t)stream);
+  a.row_tiles = (S * a.G + p.rows - 1) / p.rows;
+  PBS_REQUIRE((int64_t)B * a.row_tiles <= INT32_MAX, "pbs_paged_attn_fwd: too many query rows");
+  a.headers = p.cut ? (PagedHeader*)workspace : nullptr;
+  a.parts = p.cut ? (float*)((char*)workspace + PAGED_WORKERS * sizeof(PagedHeader)) : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.rows > 32) {
+    if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
+  } else if (kv_bits == 16) {
+    if (p.rows == 16) launch<16, 1, 1>(a, st);
+    else launch<16, 2, 1>(a, st);
+  } else {
+    if (p.rows == 16) launch<4, 1, 2>(a, st);
+    else launch<4, 2, 2>(a, st);
+  }
+  if (p.cut) hipLaunchKernelGGL(join_kernel, dim3(PAGED_WORKERS, p.rows / WAVES), dim3(256), 0, st, a, p.rows);
   return pbs_check_launch("pbs_paged_attn_fwd");
 }

@@ -41,6 +41,13 @@ __device__ __forceinline__ float sum_over_groups(float v) {
   return __uint_as_float(t.a) + __uint_as_float(t.b);
 }
 
+// lane id formed where it is asked for: what is derived from it holds no registers elsewhere
+__device__ __forceinline__ int paged_lane() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 // a sequence, and one of its row tiles
 struct PagedSeq {
   int b, past, fresh;

@@ -127,39 +127,42 @@ __device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
 }
 __device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
 
-// V^T operands: v[d] holds eight tokens (8 g ..) of channel 16 d + n, of 4-bit pages of channel 8 n + d.  `held` of the eight are there.
+// V^T operands: d's holds eight tokens (8 g ..) of channel 16 d + n, of 4-bit pages of channel 8 n + d; here d = 2 c and 2 c + 1.  `held` of the
+// eight are there.
 template <bool TAIL>
-__device__ __forceinline__ void values(const Tile<16>& t, int held, bf16x8 (&v)[8]) {
+__device__ __forceinline__ void values(const Tile<16>& t, int c, int held, bf16x8 (&v)[2]) {
 #pragma unroll
-  for (int d = 0; d < 8; ++d) {
-    u32x4 x = t.v[d];
+  for (int e = 0; e < 2; ++e) {
+    u32x4 x = t.v[2 * c + e];
     if (TAIL) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) x[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
     }
-    v[d] = __builtin_bit_cast(bf16x8, x);
+    v[e] = __builtin_bit_cast(bf16x8, x);
   }
 }
+template <int C>
+__device__ __forceinline__ uint32_t value_pair(uint32_t codes, uint32_t e) {   // channels 2 C and 2 C + 1 of a word
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(e), C));
+}
 template <bool TAIL>
-__device__ __forceinline__ void values(const Tile<4>& t, int held, bf16x8 (&v)[8]) {
-  u32x4 x[8];   // token j: channels 8 n .. 8 n + 7
+__device__ __forceinline__ void values(const Tile<4>& t, int c, int held, bf16x8 (&v)[2]) {
+  uint32_t x[8];   // token j: two channels
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     uint32_t e = (t.vs[j >> 2] >> (8 * (j & 3))) & 0xffu;
     if (TAIL) e = j < held ? e : 0u;   // (codes are finite whatever the page held before)
-    x[j] = fp4_values(t.v[j >> 2][j & 3], __uint_as_float(e << 23));
+    const uint32_t w = t.v[j >> 2][j & 3];
+    x[j] = c == 0 ? value_pair<0>(w, e << 23) : c == 1 ? value_pair<1>(w, e << 23) : c == 2 ? value_pair<2>(w, e << 23) : value_pair<3>(w, e << 23);
   }
+  u32x4 lo, hi;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    u32x4 lo, hi;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      lo[w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x05040100u);
-      hi[w] = __builtin_amdgcn_perm(x[2 * w + 1][c], x[2 * w][c], 0x07060302u);
-    }
-    v[2 * c] = __builtin_bit_cast(bf16x8, lo);
-    v[2 * c + 1] = __builtin_bit_cast(bf16x8, hi);
+  for (int w = 0; w < 4; ++w) {
+    lo[w] = __builtin_amdgcn_perm(x[2 * w + 1], x[2 * w], 0x05040100u);
+    hi[w] = __builtin_amdgcn_perm(x[2 * w + 1], x[2 * w], 0x07060302u);
   }
+  v[0] = __builtin_bit_cast(bf16x8, lo);
+  v[1] = __builtin_bit_cast(bf16x8, hi);
 }
 template <int BITS>
 __device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? d * 16 + row : row * 8 + d; }
@@ -233,13 +236,17 @@ struct Softmax {
   __device__ __forceinline__ void add(const Tile<BITS> (&t)[NT], const bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, int g) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      bf16x8 v[8];
       // tokens behind the keys hold whatever the page held before: not even times zero
-      values<TAIL>(t[i], gone >> i & 1 ? 0 : keys - k0 - i * PAGED_TILE - 8 * g, v);
+      const int held = gone >> i & 1 ? 0 : keys - k0 - i * PAGED_TILE - 8 * g;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int c = 0; c < 4; ++c) {
+        bf16x8 v[2];
+        values<TAIL>(t[i], c, held, v);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d], p[r][i], o[r][d], 0, 0, 0);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) o[r][2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[e], p[r][i], o[r][2 * c + e], 0, 0, 0);
+      }
     }
   }
 };
@@ -248,16 +255,19 @@ struct Softmax {
 template <int BITS, int R, int NT>
 __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part,
                                      float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2]) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int lane = paged_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   Softmax<BITS, R, NT> s;
   s.begin(a, u, head, n, g);
   const int tiles = (u.keys + PAGED_TILE - 1) / PAGED_TILE;
   int t = (s0 * WAVES + wave) * NT;                             // this wave's first tile of the step
   const int end = min((s0 + steps) * WAVES * NT, tiles);
-  Tile<BITS> tile[NT];
-  uint32_t gone = 0;
-  // pages are looked up a step ahead; a tile that is not there is read as the pool's first one, and not used
-  auto look_up = [&](int t, int64_t (&at)[NT]) __attribute__((always_inline)) {
+  // Loads go out DEPTH steps ahead, a step's K as soon as the K before it in the same registers has been multiplied, its V likewise.  Pages are
+  // looked up before that; a tile that is not there is read as the pool's first one, and not used.
+  constexpr int DEPTH = BITS == 4 ? 2 : 1, STRIDE = WAVES * NT;
+  Tile<BITS> tile[DEPTH][NT];
+  uint32_t gone[DEPTH] = {};
+  int64_t at[NT];
+  auto look_up = [&](int t) __attribute__((always_inline)) {
     uint32_t none = 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -267,19 +277,20 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     }
     return none;
   };
-  int64_t at[NT];
-  if (t < end) {
-    gone = look_up(t, at);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
+  for (int d = 0; d < DEPTH; ++d)
+    if (t + d * STRIDE < end) {
+      gone[d] = look_up(t + d * STRIDE);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
-  }
-  while (t < end) {
-    const int next = t + WAVES * NT, k0 = t * PAGED_TILE;
+      for (int i = 0; i < NT; ++i) load_k(tile[d][i], a.pool, at[i], n, g);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) load_v(tile[d][i], a.pool, at[i], n, g);
+    }
+  auto one = [&](Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
+    const int next = t + DEPTH * STRIDE, k0 = t * PAGED_TILE;
     const bool whole = k0 + NT * PAGED_TILE <= min(u.all_see, u.keys) && gone == 0;
     uint32_t gone_next = 0;
-    if (next < end) gone_next = look_up(next, at);
+    if (next < end) gone_next = look_up(next);
     bf16x8 p[R][NT];
     if (whole) s.template weigh<false>(tile, p, k0, u.keys, gone, a.scale_log2, g);
     else s.template weigh<true>(tile, p, k0, u.keys, gone, a.scale_log2, g);
@@ -294,29 +305,37 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
     }
     gone = gone_next;
-    t = next;
+    t += STRIDE;
+  };
+  while (t < end) {
+    one(tile[0], gone[0]);
+    if (DEPTH == 2) {
+      if (t >= end) break;
+      one(tile[DEPTH - 1], gone[DEPTH - 1]);
+    }
   }
 
+  const int lane2 = paged_lane(), n2 = lane2 & 15, g2 = lane2 >> 4;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float l = sum_over_groups(s.l[r]);
     if (r > 0) __syncthreads();   // (the rows before have been read)
-    if (g == 0) {
-      ml_lds[wave][n][0] = s.m[r];
-      ml_lds[wave][n][1] = l;
+    if (g2 == 0) {
+      ml_lds[wave][n2][0] = s.m[r];
+      ml_lds[wave][n2][1] = l;
     }
     __syncthreads();
-    float top = ml_lds[0][n][0];
+    float top = ml_lds[0][n2][0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, ml_lds[w][n][0]);
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, ml_lds[w][n2][0]);
     const float f = __builtin_amdgcn_exp2f(s.m[r] - top);
 #pragma unroll
     for (int d = 0; d < 8; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o_lds[wave][n][channel_of<BITS>(d, 4 * g + i)] = f == 0.f ? 0.f : s.o[r][d][i] * f;
+      for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = f == 0.f ? 0.f : s.o[r][d][i] * f;
     __syncthreads();
     // 16 lanes a row, 8 channels a lane
-    const int rr = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
+    const int rr = wave * 4 + g2, c = n2 * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
     float y[8], row_top = ml_lds[0][rr][0], sum = 0.f;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) row_top = fmaxf(row_top, ml_lds[w][rr][0]);
@@ -355,34 +374,63 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(PagedAttnArgs a) {
                                             __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds); });
 }
 
-// Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it, in order.  A wave a row.
+// Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it.  Sixteen lanes hold a
+// row, 8 channels each; the workgroup's sixteen such groups take GROUPS shares of a row's parts and 16 / GROUPS rows.  With few rows there are
+// many parts (128k tokens of one sequence: 65), and one group after the other through them all took 35 us.
+template <int GROUPS>
 __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
   const PagedHeader h = a.headers[blockIdx.x];
   if (h.more == 0) return;
   const int b = h.unit / a.row_tiles, fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
-  const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), row = (h.unit - b * a.row_tiles) * rows + rr, token = row / a.G;
-  if (token >= a.S) return;
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, share = group % GROUPS;
+  const int rr = blockIdx.y * (16 / GROUPS) + group / GROUPS, row = (h.unit - b * a.row_tiles) * rows + rr, token = row / a.G;
+  if (GROUPS == 16 && token >= a.S) return;
   const int slot = paged_slot_floats(rows);
   const float* first = a.parts + ((int64_t)blockIdx.x * 2 + 1) * slot;
-  // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
-  auto part = [&](int i) { return first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot); };
-  float top = -FLT_MAX;
-  for (int i = lane; i <= h.more; i += 64) top = fmaxf(top, part(i)[rows * PAGED_D + rr * 2]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-  float sum = 0.f;
-  f32x2 y = {};
+  float top = -FLT_MAX, sum = 0.f;
+  f32x4 y0 = {}, y1 = {};
+  if (token < a.S) {
 #pragma unroll 4
-  for (int i = 0; i <= h.more; ++i) {
-    const float* p = part(i);
-    const f32x2 ml = *(const f32x2*)(p + rows * PAGED_D + rr * 2), x = *(const f32x2*)(p + rr * PAGED_D + lane * 2);
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    sum += ml.y * f;
-    if (f != 0.f) y += x * f;
+    for (int i = share; i <= h.more; i += GROUPS) {
+      // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
+      const float* p = first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot);
+      const f32x2 ml = *(const f32x2*)(p + rows * PAGED_D + rr * 2);
+      const f32x4 x0 = *(const f32x4*)(p + rr * PAGED_D + lane * 8), x1 = *(const f32x4*)(p + rr * PAGED_D + lane * 8 + 4);
+      const float m = fmaxf(top, ml.x), old = __builtin_amdgcn_exp2f(top - m), now = __builtin_amdgcn_exp2f(ml.x - m);
+      top = m;
+      sum = sum * old + ml.y * now;
+      y0 = (old == 0.f ? (f32x4){} : y0 * old) + (now == 0.f ? (f32x4){} : x0 * now);
+      y1 = (old == 0.f ? (f32x4){} : y1 * old) + (now == 0.f ? (f32x4){} : x1 * now);
+    }
   }
+  if (GROUPS > 1) {
+    __shared__ float y_lds[16][16][8], ml_lds[16][2];
+    *(f32x4*)y_lds[group][lane] = y0;
+    *(f32x4*)(y_lds[group][lane] + 4) = y1;
+    if (lane == 0) {
+      ml_lds[group][0] = top;
+      ml_lds[group][1] = sum;
+    }
+    __syncthreads();
+    if (share != 0) return;
+    for (int w = 0; w < GROUPS; ++w) top = fmaxf(top, ml_lds[group + w][0]);
+    sum = 0.f;
+    y0 = y1 = (f32x4){};
+#pragma unroll
+    for (int w = 0; w < GROUPS; ++w) {
+      const float f = __builtin_amdgcn_exp2f(ml_lds[group + w][0] - top);
+      sum += ml_lds[group + w][1] * f;
+      if (f != 0.f) {
+        y0 += *(const f32x4*)y_lds[group + w][lane] * f;
+        y1 += *(const f32x4*)(y_lds[group + w][lane] + 4) * f;
+      }
+    }
+  }
+  if (token >= a.S) return;
   const float scale = sum == 0.f || token >= fresh ? 0.f : 1.f / sum;
-  const uint32_t w = scale == 0.f ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){y.x * scale, y.y * scale}, bf16x2));
-  *(uint32_t*)(a.out + b * a.o_sb + (h.head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + lane * 2) = w;
+  auto two = [&](float x, float y) { return scale == 0.f ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x * scale, y * scale}, bf16x2)); };
+  *(u32x4*)(a.out + b * a.o_sb + (h.head * a.G + row % a.G) * a.o_sh + (int64_t)token * a.o_ss + lane * 8) =
+      (u32x4){two(y0[0], y0[1]), two(y0[2], y0[3]), two(y1[0], y1[1]), two(y1[2], y1[3])};
 }
 
 struct Plan {
@@ -450,6 +498,9 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
     if (p.rows == 16) launch<4, 1, 2>(a, st);
     else launch<4, 2, 2>(a, st);
   }
-  if (p.cut) hipLaunchKernelGGL(join_kernel, dim3(PAGED_WORKERS, p.rows / WAVES), dim3(256), 0, st, a, p.rows);
+  if (p.cut) {
+    if (p.rows <= 32) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
+    else hipLaunchKernelGGL(join_kernel<1>, dim3(PAGED_WORKERS, p.rows / 16), dim3(256), 0, st, a, p.rows);
+  }
   return pbs_check_launch("pbs_paged_attn_fwd");
 }

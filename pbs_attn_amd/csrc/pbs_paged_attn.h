@@ -7,6 +7,9 @@
 constexpr int PAGED_WAVES = 4;       // of a workgroup
 constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences: two a compute unit
 constexpr int PAGED_LEAST_STEPS = 2;   // steps that a worker takes at least
+// A row's exponent is taken up where a logit is more than this above it (log2): weights stay below 2^8, which costs their sums in fp32 and their
+// roundings to bf16 nothing, and the sums are rescaled a few times in a sequence rather than with every new maximum.
+constexpr float PAGED_SLACK = 8.f;
 
 struct PagedHeader {   // of a worker: the piece of work that it began and left to the `more` workers after it
   int unit, head, more, pad;

@@ -6,6 +6,7 @@
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -56,9 +57,21 @@ __device__ __forceinline__ void load_v(Tile<4>& t, const PagedPool& p, int64_t a
 // 16 query rows as the matrix instruction's right operand
 template <int BITS>
 struct Rows;
+struct RowsLds {   // of the four waves, lane by lane
+  u32x4 q[4][64];
+  int scale[64];
+};
 template <>
 struct Rows<16> {
   bf16x8 q[4];
+  __device__ __forceinline__ void put(RowsLds& lds, int lane) const {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) lds.q[c][lane] = __builtin_bit_cast(u32x4, q[c]);
+  }
+  __device__ __forceinline__ void get(const RowsLds& lds, int lane) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q[c] = __builtin_bit_cast(bf16x8, lds.q[c][lane]);
+  }
   __device__ __forceinline__ void load(const uint16_t* row, int g) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -74,7 +87,25 @@ struct Rows<16> {
 template <>
 struct Rows<4> {
   i32x8 hi, lo;
-  int scale_hi, scale_lo;
+  int scale_hi;
+  __device__ __forceinline__ int scale_lo() const { return scale_hi == 255 ? 255 : scale_hi - 5; }
+  __device__ __forceinline__ void put(RowsLds& lds, int lane) const {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      lds.q[c][lane] = (u32x4){(uint32_t)hi[4 * c], (uint32_t)hi[4 * c + 1], (uint32_t)hi[4 * c + 2], (uint32_t)hi[4 * c + 3]};
+      lds.q[2 + c][lane] = (u32x4){(uint32_t)lo[4 * c], (uint32_t)lo[4 * c + 1], (uint32_t)lo[4 * c + 2], (uint32_t)lo[4 * c + 3]};
+    }
+    lds.scale[lane] = scale_hi;
+  }
+  __device__ __forceinline__ void get(const RowsLds& lds, int lane) {
+    const u32x4 a = lds.q[0][lane], b = lds.q[1][lane], c = lds.q[2][lane], d = lds.q[3][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi[e] = (int)a[e]; hi[4 + e] = (int)b[e];
+      lo[e] = (int)c[e]; lo[4 + e] = (int)d[e];
+    }
+    scale_hi = lds.scale[lane];
+  }
   __device__ __forceinline__ void load(const uint16_t* row, int g) {
     u32x4 x[4] = {};   // channels 16 g .. 16 g + 15 and 64 + 16 g ..: 32 bytes of an 8-bit operand
     if (row) {
@@ -107,7 +138,6 @@ struct Rows<4> {
       lo[w] = l;
     }
     scale_hi = field >= 255 ? 255 : field - 7;    // (an infinity or NaN among the queries: NaN)
-    scale_lo = field >= 255 ? 255 : field - 12;
   }
 };
 
@@ -122,7 +152,7 @@ template <int HALF>
 __device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
   const i32x8 k = {(int)t.k[HALF][0], (int)t.k[HALF][1], (int)t.k[HALF][2], (int)t.k[HALF][3], 0, 0, 0, 0};
   f32x4 s = {};
-  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo);
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo());
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 4, 0, HALF, (int)t.ks, 0, r.scale_hi);
 }
 __device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
@@ -171,63 +201,84 @@ __device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? 
 // its share of P^T in O^T += V^T P^T: probabilities never change lanes.
 template <int BITS, int R, int NT>
 struct Softmax {
-  Rows<BITS> rows[R];
+  // The queries stay in registers where a wave has one row tile, and in LDS otherwise: 16 registers each (bf16, 35 rows: 256 and 138 spilled)
+  Rows<BITS> own;
+  RowsLds* lds;
   f32x4 o[R][8];
   float m[R], l[R];
   int seen[R];
 
-  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedUnit& u, int head, int n, int g) {
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedUnit& u, int head, int n, int g, int wave, RowsLds* q_lds) {
+    lds = q_lds;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = u.r0 + r * 16 + n, token = row / a.G;
       const bool valid = token < u.fresh;
-      rows[r].load(valid ? a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss : nullptr, g);
+      if (R == 1 || wave == r % PAGED_WAVES) {
+        own.load(valid ? a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss : nullptr, g);
+        if (R > 1) own.put(lds[r], g * 16 + n);
+      }
       seen[r] = valid ? u.past + token + 1 : 0;
       m[r] = -FLT_MAX;
       l[r] = 0.f;
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[r][d] = (f32x4){};
     }
+    if (R > 1) __syncthreads();
   }
   // logits of the NT tiles; `k0`: the first one's first key, `keys`: how many there are, bit i of `gone`: tile i's page is not there
   template <bool MASK>
-  __device__ __forceinline__ void weigh(const Tile<BITS> (&t)[NT], bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, float c, int g) {
+  __device__ __forceinline__ void weigh(const Tile<BITS> (&t)[NT], bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, float c, int n, int g) {
+    if (R > 1) asm volatile("" ::: "memory");   // (or all queries are read ahead of the loop, into registers)
+    // (all row tiles' products first, then one decision: nothing waits for a row tile's maximum)
+    float x[R][NT][8], top[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float x[NT][8];
+      if (R > 1) own.get(lds[r], g * 16 + n);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const f32x4 s0 = logits(t[i], 0, rows[r]), s1 = logits(t[i], 1, rows[r]);
+        const f32x4 s0 = logits(t[i], 0, own), s1 = logits(t[i], 1, own);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[i][j] = (j & 1) ? s1[j >> 1] : s0[j >> 1];
+          x[r][i][j] = (j & 1) ? s1[j >> 1] : s0[j >> 1];
           if (MASK) {
             const int key = k0 + i * PAGED_TILE + 8 * g + j;
-            x[i][j] = key < min(seen[r], keys) && !(gone >> i & 1) ? x[i][j] : -INFINITY;
+            x[r][i][j] = key < min(seen[r], keys) && !(gone >> i & 1) ? x[r][i][j] : -INFINITY;
           }
         }
       }
-      float top = x[0][0];
+    }
+    bool grows = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      top[r] = x[r][0][0];
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, x[i][j]);
-      const float m_new = fmaxf(m[r], max_over_groups(top) * c);
-      if (__any(m_new > m[r])) {
-        const float f = __builtin_amdgcn_exp2f(m[r] - m_new);
+        for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], x[r][i][j]);
+      top[r] = max_over_groups(top[r]) * c;
+      grows |= top[r] > m[r] + PAGED_SLACK;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float m_new = fmaxf(m[r], top[r]), f = __builtin_amdgcn_exp2f(m[r] - m_new);
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;
         m[r] = m_new;
       }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], c, -m[r]));
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i][j], c, -m[r]));
           sum += e;
-          p[r][i][j] = (__bf16)e;   // (weights of at most 1, half a step of 2^-8 off: they are summed as they are, and multiply bf16 values)
+          p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
         }
       l[r] += sum;
     }
@@ -254,16 +305,16 @@ struct Softmax {
 // Steps `s0` .. `s0 + steps - 1` of a unit and head, 4 * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
 template <int BITS, int R, int NT>
 __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part,
-                                     float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2]) {
+                                     float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2], RowsLds* q_lds) {
   const int lane = paged_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   Softmax<BITS, R, NT> s;
-  s.begin(a, u, head, n, g);
+  s.begin(a, u, head, n, g, wave, q_lds);
   const int tiles = (u.keys + PAGED_TILE - 1) / PAGED_TILE;
   int t = (s0 * WAVES + wave) * NT;                             // this wave's first tile of the step
   const int end = min((s0 + steps) * WAVES * NT, tiles);
   // Loads go out DEPTH steps ahead, a step's K as soon as the K before it in the same registers has been multiplied, its V likewise.  Pages are
   // looked up before that; a tile that is not there is read as the pool's first one, and not used.
-  constexpr int DEPTH = BITS == 4 ? 2 : 1, STRIDE = WAVES * NT;
+  constexpr int DEPTH = NT == 2 ? 2 : 1, STRIDE = WAVES * NT;
   Tile<BITS> tile[DEPTH][NT];
   uint32_t gone[DEPTH] = {};
   int64_t at[NT];
@@ -277,43 +328,64 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     }
     return none;
   };
+  if (t < end) {
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (t + d * STRIDE < end) {
+    for (int d = 0; d < DEPTH; ++d) {
+      if (t + d * STRIDE >= end) break;
       gone[d] = look_up(t + d * STRIDE);
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[d][i], a.pool, at[i], n, g);
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_v(tile[d][i], a.pool, at[i], n, g);
     }
-  auto one = [&](Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
+  }
+  auto one = [&](auto mask, Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
     const int next = t + DEPTH * STRIDE, k0 = t * PAGED_TILE;
-    const bool whole = k0 + NT * PAGED_TILE <= min(u.all_see, u.keys) && gone == 0;
+    // (with several row tiles the loads behind the last step repeat its own: without the branches 35 rows take 68 us for 73; with one row
+    // tile the steps are short, and the wait for what nobody uses costs 2 %)
+    const bool load = R > 1 || next < end;
     uint32_t gone_next = 0;
-    if (next < end) gone_next = look_up(next);
+    if (load) gone_next = look_up(R == 1 || next < end ? next : t);
     bf16x8 p[R][NT];
-    if (whole) s.template weigh<false>(tile, p, k0, u.keys, gone, a.scale_log2, g);
-    else s.template weigh<true>(tile, p, k0, u.keys, gone, a.scale_log2, g);
-    if (next < end) {
+    s.template weigh<mask.value>(tile, p, k0, u.keys, gone, a.scale_log2, n, g);
+    if (load) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
     }
-    if (whole) s.template add<false>(tile, p, k0, u.keys, gone, g);
-    else s.template add<true>(tile, p, k0, u.keys, gone, g);
-    if (next < end) {
+    s.template add<mask.value>(tile, p, k0, u.keys, gone, g);
+    if (load) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
     }
     gone = gone_next;
     t += STRIDE;
   };
-  while (t < end) {
-    one(tile[0], gone[0]);
-    if (DEPTH == 2) {
-      if (t >= end) break;
-      one(tile[DEPTH - 1], gone[DEPTH - 1]);
+  // (tiles that every row sees whole, then the rest: those at the end, and whatever follows a page that is not there)
+  const int seen_whole = min(u.all_see, u.keys) / PAGED_TILE - NT;
+  auto loop = [&](auto mask) __attribute__((always_inline)) {
+    while (t < end) {
+      if (!mask.value && (t > seen_whole || gone[0] != 0)) break;
+      one(mask, tile[0], gone[0]);
+      if (DEPTH == 2) {
+        if (t < end && (mask.value || (t <= seen_whole && gone[DEPTH - 1] == 0))) {
+          one(mask, tile[DEPTH - 1], gone[DEPTH - 1]);
+        } else {   // the buffers change places
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const Tile<BITS> x = tile[0][i];
+            tile[0][i] = tile[DEPTH - 1][i];
+            tile[DEPTH - 1][i] = x;
+          }
+          const uint32_t y = gone[0];
+          gone[0] = gone[DEPTH - 1];
+          gone[DEPTH - 1] = y;
+          break;
+        }
+      }
     }
-  }
+  };
+  loop(std::false_type{});
+  loop(std::true_type{});
 
   const int lane2 = paged_lane(), n2 = lane2 & 15, g2 = lane2 >> 4;
 #pragma unroll
@@ -370,8 +442,9 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(PagedAttnArgs a) {
   __shared__ float o_lds[WAVES][16][O_PITCH];
   __shared__ float ml_lds[WAVES][16][2];
   __shared__ PagedShareLds share_lds;
+  __shared__ RowsLds q_lds[R > 1 ? R : 1];
   paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, blockIdx.y, [&](const PagedUnit& u, int head, int step, int steps, float* part)
-                                            __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds); });
+                                            __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds); });
 }
 
 // Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it.  Sixteen lanes hold a
@@ -441,9 +514,9 @@ struct Plan {
 Plan plan_of(int B, int Hq, int Hkv, int S, int max_len) {
   Plan p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : rows <= 64 ? 64 : 128;
   const int64_t units = B * ((rows + p.rows - 1) / p.rows);
-  p.cut = max_len > 512 && (p.rows <= 32 || units * Hkv < 4 * PAGED_WORKERS);
+  p.cut = max_len > 512 && (p.rows <= 48 || units * Hkv < 4 * PAGED_WORKERS);
   if (units > 65535) p.cut = true;   // (a grid's second index)
   p.bytes = p.cut ? PAGED_WORKERS * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows)) : 0;
   return p;
@@ -489,17 +562,19 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.headers = p.cut ? (PagedHeader*)workspace : nullptr;
   a.parts = p.cut ? (float*)((char*)workspace + PAGED_WORKERS * sizeof(PagedHeader)) : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  if (p.rows > 32) {
+  if (p.rows > 48) {
     if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
   } else if (kv_bits == 16) {
     if (p.rows == 16) launch<16, 1, 1>(a, st);
-    else launch<16, 2, 1>(a, st);
+    else if (p.rows == 32) launch<16, 2, 1>(a, st);
+    else launch<16, 3, 1>(a, st);
   } else {
     if (p.rows == 16) launch<4, 1, 2>(a, st);
-    else launch<4, 2, 2>(a, st);
+    else if (p.rows == 32) launch<4, 2, 1>(a, st);
+    else launch<4, 3, 1>(a, st);
   }
   if (p.cut) {
-    if (p.rows <= 32) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
+    if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
     else hipLaunchKernelGGL(join_kernel<1>, dim3(PAGED_WORKERS, p.rows / 16), dim3(256), 0, st, a, p.rows);
   }
   return pbs_check_launch("pbs_paged_attn_fwd");

@@ -203,21 +203,30 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
           }
     }
     bf16x8 p[RW][2];
+    float top[RW];
+    bool grows = false;
 #pragma unroll
     for (int r = 0; r < RW; ++r) {
-      float top = s[r][0][0][0];
+      top[r] = s[r][0][0][0];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[r][i][j & 1][j >> 1]);
-      const float m_new = fmaxf(m[r], max_over_groups(top) * c);
-      if (__any(m_new > m[r])) {
-        const float f = __builtin_amdgcn_exp2f(m[r] - m_new);
+        for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], s[r][i][j & 1][j >> 1]);
+      top[r] = max_over_groups(top[r]) * c;
+      grows |= top[r] > m[r] + PAGED_SLACK;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const float m_new = fmaxf(m[r], top[r]), f = __builtin_amdgcn_exp2f(m[r] - m_new);
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;
         m[r] = m_new;
       }
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -225,7 +234,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         for (int j = 0; j < 8; ++j) {
           const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
           sum += e;
-          p[r][i][j] = (__bf16)e;   // (weights of at most 1, half a step of 2^-8 off: they are summed as they are, and multiply bf16 values)
+          p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
         }
       l[r] += sum;
     }

@@ -55,7 +55,7 @@ __device__ __forceinline__ int paged_lane() {
 struct PagedSeq {
   int b, past, fresh;
   int steps;         // of a row tile with tokens (the last one's: tiles before it see fewer keys, and idle for a while)
-  int64_t a_head;    // steps of one head: row tiles without tokens take one, in which their rows are cleared
+  int a_head;        // steps of one head: row tiles without tokens take one, in which their rows are cleared
   int tiles;         // row tiles with tokens
 };
 template <int ROWS, int STEP>
@@ -66,7 +66,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b) {
   s.fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
   s.tiles = (s.fresh * a.G + ROWS - 1) / ROWS;
   s.steps = max((min(s.past + s.fresh, a.pool.max_pages << a.pool.page_shift) + STEP - 1) / STEP, 1);
-  s.a_head = (int64_t)s.tiles * s.steps + (a.row_tiles - s.tiles);
+  s.a_head = s.tiles * s.steps + (a.row_tiles - s.tiles);
   return s;
 }
 struct PagedUnit {
@@ -86,81 +86,94 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedAttnArgs& a, int b, i
 }
 
 // Where a workgroup begins, and how many steps are its.  The steps of all sequences lie in one line (sequence, head, row tile, step), cut
-// into equal shares, one a worker, so that sequences of any lengths fill the chip.
+// into equal shares, one a worker, so that sequences of any lengths fill the chip.  (The host sees to it that the line's length fits 32 bits.)
 struct PagedShare {
-  int worker, b, head, tile, step;
-  int64_t todo, share;
+  int b, head, tile, step, todo, share;
 };
 struct PagedShareLds {
-  int64_t wave_sums[PAGED_WAVES], left;
-  int b;
+  int wave_sums[PAGED_WAVES], left, b;
 };
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int workers, PagedShare* out) {
-  const int tid = threadIdx.x, stretch = (a.B + 255) / 256, from = min(tid * stretch, a.B), to = min(from + stretch, a.B);
-  int64_t mine = 0;
-  for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
-  int64_t before = mine;
+  int total = 0, before = 0, mine = 0, from = 0;
+  if (a.B == 1) {
+    total = a.Hkv * paged_seq<ROWS, STEP>(a, 0).a_head;
+  } else {   // running sums over the sequences, a stretch of them a thread
+    const int tid = threadIdx.x, stretch = (a.B + 255) / 256, to = min((tid + 1) * stretch, a.B);
+    from = min(tid * stretch, a.B);
+    for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+    before = mine;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t other = __shfl_up(before, d, 64);
-    if ((tid & 63) >= d) before += other;
-  }
-  if ((tid & 63) == 63) lds.wave_sums[tid >> 6] = before;
-  before -= mine;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < PAGED_WAVES; ++w) {
-    if (w < (tid >> 6)) before += lds.wave_sums[w];
-    total += lds.wave_sums[w];
-  }
-  out->worker = worker;
-  out->share = max((total + workers - 1) / workers, (int64_t)PAGED_LEAST_STEPS);
-  const int64_t start = out->share * worker;
-  out->todo = min(out->share, total - start);
-  if (start >= total) return false;
-  if (start >= before && start < before + mine) {
-    int64_t left = start - before;
-    for (int i = from;; ++i) {
-      const int64_t cost = a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
-      if (left < cost) {
-        lds.b = i;
-        lds.left = left;
-        break;
-      }
-      left -= cost;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = __shfl_up(before, d, 64);
+      if ((tid & 63) >= d) before += other;
     }
+    if ((tid & 63) == 63) lds.wave_sums[tid >> 6] = before;
+    before -= mine;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PAGED_WAVES; ++w) {
+      if (w < (tid >> 6)) before += lds.wave_sums[w];
+      total += lds.wave_sums[w];
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
   }
-  __syncthreads();
-  const PagedSeq s = paged_seq<ROWS, STEP>(a, __builtin_amdgcn_readfirstlane(lds.b));
-  const int64_t head = lds.left / s.a_head, left = lds.left - head * s.a_head, full = (int64_t)s.tiles * s.steps;
-  out->b = s.b;
-  out->head = __builtin_amdgcn_readfirstlane((int)head);
-  out->tile = __builtin_amdgcn_readfirstlane((int)(left < full ? left / s.steps : s.tiles + (left - full)));
-  out->step = __builtin_amdgcn_readfirstlane((int)(left < full ? left % s.steps : 0));
+  const int share = max((int)(((unsigned)total + workers - 1) / workers), PAGED_LEAST_STEPS);
+  if ((int64_t)share * worker >= total) return false;
+  const int start = share * worker;
+  out->share = share;
+  out->todo = min(share, total - start);
+  int b = 0, left = start;
+  if (a.B > 1) {
+    if (start >= before && start < before + mine) {
+      left = start - before;
+      for (int i = from;; ++i) {
+        const int cost = a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+        if (left < cost) {
+          lds.b = i;
+          lds.left = left;
+          break;
+        }
+        left -= cost;
+      }
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(lds.b);
+    left = __builtin_amdgcn_readfirstlane(lds.left);
+  }
+  const PagedSeq s = paged_seq<ROWS, STEP>(a, b);
+  const int full = s.tiles * s.steps;
+  out->b = b;
+  out->head = left / s.a_head;
+  left -= out->head * s.a_head;
+  out->tile = left < full ? left / s.steps : s.tiles + (left - full);
+  out->step = left < full ? left - out->tile * s.steps : 0;
   return true;
 }
 
 // A workgroup's way through its share, or through the one row tile and head that are its without headers: work(unit, head, first step,
 // steps, part), part null where the steps are all that the row tile has.
 template <int ROWS, int STEP, class Work>
-__device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int tile, Work&& work) {
+__device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& lds, int worker, bool last_tile_first, Work&& work) {
   PagedShare at;
-  at.worker = worker; at.b = tile / a.row_tiles; at.head = blockIdx.x; at.tile = tile - at.b * a.row_tiles; at.step = 0;
-  at.share = at.todo = INT32_MAX;
-  if (a.headers && !paged_share<ROWS, STEP>(a, lds, worker, gridDim.x, &at)) {
-    if (threadIdx.x == 0) a.headers[worker].more = 0;
-    return;
+  if (a.headers) {
+    if (!paged_share<ROWS, STEP>(a, lds, worker, gridDim.x, &at)) {
+      if (threadIdx.x == 0) a.headers[worker].more = 0;
+      return;
+    }
+  } else {
+    const int unit = blockIdx.x / a.Hkv, tile = unit % a.row_tiles;
+    at.b = unit / a.row_tiles; at.head = blockIdx.x % a.Hkv; at.tile = last_tile_first ? a.row_tiles - 1 - tile : tile; at.step = 0;
+    at.share = at.todo = INT32_MAX;
   }
   int more = 0;
   PagedSeq s = paged_seq<ROWS, STEP>(a, at.b);
   while (true) {
-    const int steps = at.tile < s.tiles ? s.steps : 1, n = (int)min((int64_t)(steps - at.step), at.todo);
+    const int steps = at.tile < s.tiles ? s.steps : 1, n = min(steps - at.step, at.todo);
     at.todo -= n;
     float* part = nullptr;
     if (n < steps) part = a.parts + ((int64_t)worker * 2 + (at.step == 0)) * paged_slot_floats(ROWS);
-    if (at.step == 0 && n < steps) more = (int)((steps - n + at.share - 1) / at.share);
+    if (at.step == 0 && n < steps) more = (int)((unsigned)(steps - n + at.share - 1) / (unsigned)at.share);
     work(paged_unit<ROWS>(a, s.b, s.past, s.fresh, at.tile), at.head, at.step, n, part);
     if (!a.headers) return;
     if (at.todo == 0) break;

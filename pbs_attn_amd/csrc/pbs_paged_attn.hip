@@ -443,7 +443,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(PagedAttnArgs a) {
   __shared__ float ml_lds[WAVES][16][2];
   __shared__ PagedShareLds share_lds;
   __shared__ RowsLds q_lds[R > 1 ? R : 1];
-  paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, blockIdx.y, [&](const PagedUnit& u, int head, int step, int steps, float* part)
+  paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, false, [&](const PagedUnit& u, int head, int step, int steps, float* part)
                                             __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds); });
 }
 
@@ -506,6 +506,9 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
       (u32x4){two(y0[0], y0[1]), two(y0[2], y0[3]), two(y1[0], y1[1]), two(y1[2], y1[3])};
 }
 
+// Steps of a row tile of `rows`
+constexpr int step_of(int rows, int kv_bits) { return rows > 48 ? 64 : rows == 16 && kv_bits == 4 ? 256 : 128; }
+
 struct Plan {
   int rows;   // of a row tile
   bool cut;
@@ -515,16 +518,14 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int max_len) {
   Plan p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : rows <= 64 ? 64 : 128;
-  const int64_t units = B * ((rows + p.rows - 1) / p.rows);
-  p.cut = max_len > 512 && (p.rows <= 48 || units * Hkv < 4 * PAGED_WORKERS);
-  if (units > 65535) p.cut = true;   // (a grid's second index)
+  p.cut = max_len > 512 && (p.rows <= 48 || B * ((rows + p.rows - 1) / p.rows) * Hkv < 4 * PAGED_WORKERS);
   p.bytes = p.cut ? PAGED_WORKERS * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows)) : 0;
   return p;
 }
 
 template <int BITS, int R, int NT>
 void launch(const PagedAttnArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), a.headers ? dim3(PAGED_WORKERS) : dim3(a.Hkv, a.B * a.row_tiles), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(a.headers ? PAGED_WORKERS : a.Hkv * a.B * a.row_tiles), dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -550,7 +551,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   PBS_REQUIRE(softmax_scale > 0.f && softmax_scale <= FLT_MAX, "pbs_paged_attn_fwd: softmax_scale must be positive and finite");
   PBS_REQUIRE(((q_sb | q_sh | q_ss | o_sb | o_sh | o_ss) % 8) == 0, "pbs_paged_attn_fwd: strides must keep rows 16-byte aligned");
   PBS_REQUIRE((((uintptr_t)q | (uintptr_t)out) % 16) == 0, "pbs_paged_attn_fwd: pointers must be 16-byte aligned");
-  const Plan p = plan_of(B, Hq, Hkv, S, max_len);
+  Plan p = plan_of(B, Hq, Hkv, S, max_len);
   PBS_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace % 256) == 0 && workspace_bytes >= p.bytes),
               "pbs_paged_attn_fwd: workspace of %zu bytes, 256-byte aligned, needed", p.bytes);
   a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.past = past_lens; a.fresh = new_lens;
@@ -558,7 +559,10 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.q_sb = q_sb; a.q_sh = q_sh; a.q_ss = q_ss; a.o_sb = o_sb; a.o_sh = o_sh; a.o_ss = o_ss;
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
   a.row_tiles = (S * a.G + p.rows - 1) / p.rows;
-  PBS_REQUIRE((int64_t)B * a.row_tiles <= INT32_MAX, "pbs_paged_attn_fwd: too many query rows");
+  const int64_t units = (int64_t)B * Hkv * a.row_tiles;
+  PBS_REQUIRE(units < (1 << 24), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
+  // the line of steps that workers share has to fit 32 bits, whatever the lengths are (units of two thirds of a million keys each fill the chip)
+  if (units * (((int64_t)max_pages * page_size + 63) / step_of(p.rows, kv_bits) + 1) > INT32_MAX) p.cut = false;
   a.headers = p.cut ? (PagedHeader*)workspace : nullptr;
   a.parts = p.cut ? (float*)((char*)workspace + PAGED_WORKERS * sizeof(PagedHeader)) : nullptr;
   hipStream_t st = (hipStream_t)stream;
@@ -574,7 +578,8 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
     else launch<4, 3, 1>(a, st);
   }
   if (p.cut) {
-    if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
+    if (p.rows == 16) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
+    else if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<4>, dim3(PAGED_WORKERS, p.rows / 4), dim3(256), 0, st, a, p.rows);
     else hipLaunchKernelGGL(join_kernel<1>, dim3(PAGED_WORKERS, p.rows / 16), dim3(256), 0, st, a, p.rows);
   }
   return pbs_check_launch("pbs_paged_attn_fwd");

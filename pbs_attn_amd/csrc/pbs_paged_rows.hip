@@ -290,9 +290,9 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 template <int BITS, int RW>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(PagedAttnArgs a) {
   // Workers that follow each other read the same head's keys at the same time: they go to one of the eight dies and its L2 (workgroups
-  // are dealt to them in turn).  Without cuts the head is the launch's first index, and the row tiles that see the most keys come first.
+  // are dealt to them in turn).  Without cuts the heads follow each other, and the row tiles that see the most keys come first.
   const int worker = a.headers ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : 0;
-  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, (int)(gridDim.y - 1 - blockIdx.y),
+  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true,
                                   [&](const PagedUnit& u, int head, int step, int steps, float* part)
                                   __attribute__((always_inline)) { work<BITS, RW>(a, u, head, step, steps, part); });
 }
@@ -305,7 +305,7 @@ int launch(const PagedAttnArgs& a, hipStream_t stream) {
     pbs_set_error("pbs_paged_attn_fwd: hipFuncSetAttribute: %s", hipGetErrorString(e));
     return (int)e;
   }
-  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), a.headers ? dim3(PAGED_WORKERS) : dim3(a.Hkv, a.B * a.row_tiles), dim3(256), LDS_TOTAL, stream, a);
+  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), dim3(a.headers ? PAGED_WORKERS : a.Hkv * a.B * a.row_tiles), dim3(256), LDS_TOTAL, stream, a);
   return 0;
 }
 

@@ -9,6 +9,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 # named after the interpreter it is built for: another one looks for a file of its own
 HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_pbs_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+PAGED_HOST_PATH = os.path.join(os.path.dirname(HOST_PATH), "_pbs_paged" + sysconfig.get_config_var("EXT_SUFFIX"))
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libpbs_hip.so")
 
 # name -> (restype, argtypes); mirrors include/pbs_hip.h
@@ -52,6 +53,7 @@ NOT_ONE_LAUNCH = -3   # PBS_NOT_ONE_LAUNCH
 
 _lib = None
 _one_segment = None
+_paged_host = None
 
 
 class PbsHipError(RuntimeError):
@@ -104,6 +106,38 @@ def one_segment():
         host.setup(torch.Tensor, torch.bfloat16, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, check, address)
         _one_segment = host.one_segment
     return _one_segment
+
+
+class _no_paged_host:
+    """In the place of the module: no call is taken."""
+    append = attn = read = pages_ok = staticmethod(_never_native)
+
+
+def paged_host():
+    """The native calls on a paged cache (csrc/pbs_paged_host.cpp): each returns None where the general path has to take the call.  Where the
+    module is missing or does not fit this interpreter and torch that is every call: the same kernels, some 10 us later."""
+    global _paged_host
+    if _paged_host is None:
+        import importlib.util
+
+        import torch
+
+        from .paged import KVPages
+        lib = load()
+        try:
+            spec = importlib.util.spec_from_file_location("_pbs_paged", PAGED_HOST_PATH)
+            host = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(host)
+        except ImportError as e:
+            import warnings
+            _paged_host = _no_paged_host
+            warnings.warn(f"calls on a paged cache go through Python: build the native ones with `python -m pbs_attn_amd.build` ({e})")
+            return _paged_host
+        addresses = [ctypes.cast(getattr(lib, name), c_void_p).value for name in
+                     ("pbs_paged_append", "pbs_paged_attn_workspace_bytes", "pbs_paged_attn_fwd", "pbs_paged_read")]
+        host.setup(KVPages, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, check, *addresses)
+        _paged_host = host
+    return _paged_host
 
 
 def check(code: int, what: str):

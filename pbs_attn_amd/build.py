@@ -72,6 +72,23 @@ def build_host_module() -> str:
     return HOST_PATH
 
 
+PAGED_HOST_SRC = os.path.join(CSRC, "pbs_paged_host.cpp")
+PAGED_HOST_PATH = os.path.join(LIB_DIR, "_pbs_paged" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_paged_host_module() -> str:
+    """Compiles the CPython module of the calls on a paged cache against the torch that is installed (no HIP headers: it is handed the
+    library's functions)."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    os.makedirs(LIB_DIR, exist_ok=True)
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + sysconfig.get_path("include"),
+                    "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", PAGED_HOST_SRC, "-o", PAGED_HOST_PATH,
+                    "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], check=True)
+    return PAGED_HOST_PATH
+
+
 C_SMOKE_SRC = os.path.join(os.path.dirname(HERE), "tests", "c_abi", "smoke.c")
 C_SMOKE_BIN = os.path.join(os.path.dirname(HERE), "tests", "c_abi", "smoke")
 
@@ -91,4 +108,5 @@ def build_c_smoke() -> str:
 if __name__ == "__main__":
     print(build_library(verbose=True))
     print(build_host_module())
+    print(build_paged_host_module())
     print(build_c_smoke())

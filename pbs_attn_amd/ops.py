@@ -393,6 +393,7 @@ def rope_qk(q, k, cos, sin):
 def _check_paged(pages, page_table, B, Hkv, lens, *ts):
     """What every call on a paged cache checks; returns the arguments that describe the pages."""
     _check_bf16_cuda(*ts)
+    pages.check()
     k = pages.k
     n, heads, page_size, _ = k.shape
     device = k.device
@@ -427,6 +428,9 @@ def paged_append(pages, page_table, past_lens, k, v, q=None, cos=None, sin=None,
     Returns (q, k) rotated, contiguous and head-major, all S rows: q (B, Hq, S, 128) where one is given, k with ``want_k``, else None.
 
     Tokens whose page is not in the pool or that lie behind the table are not stored.  At most one sequence may write to a page."""
+    done = (_lib._paged_host or _lib.paged_host()).append(pages, page_table, past_lens, k, v, q, cos, sin, new_lens, want_k)
+    if done is not None:
+        return done
     B, Hkv, S, D = k.shape
     assert v.shape == k.shape and D == HEAD_DIM
     assert q is None or (q.dim() == 4 and q.shape[0] == B and q.shape[2:] == (S, D))
@@ -465,6 +469,9 @@ def paged_append(pages, page_table, past_lens, k, v, q=None, cos=None, sin=None,
 def paged_read(pages, page_table, lens, max_len):
     """The first ``lens[b]`` tokens of every sequence of a paged cache: (k, v), each (B, Hkv, max_len, 128) bf16, contiguous; rows from
     ``lens[b]`` on are zeros, as are the tokens of pages that are not in the pool."""
+    done = (_lib._paged_host or _lib.paged_host()).read(pages, page_table, lens, max_len)
+    if done is not None:
+        return done
     B, Hkv = page_table.shape[0], pages.k.shape[1]
     n, max_pages, page_size, bits = _check_paged(pages, page_table, B, Hkv, (lens,))
     if max_len <= 0:
@@ -486,6 +493,9 @@ def paged_attn(q, pages, page_table, past_lens, new_lens=None, softmax_scale=Non
     (``paged_append``): query i of sequence b sees its tokens 0 .. ``past_lens[b] + i``.  Returns (B, Hq, S, 128); rows from
     ``new_lens[b]`` on (None: S) and rows that see no key are zeros.  ``max_len``: a length that no sequence exceeds, the new tokens
     included, where the caller knows one (default: what the table has room for); it decides how the work is cut up, not the result's meaning."""
+    out = (_lib._paged_host or _lib.paged_host()).attn(q, pages, page_table, past_lens, new_lens, softmax_scale, max_len)
+    if out is not None:
+        return out
     B, Hq, S, D = q.shape
     Hkv = pages.k.shape[1]
     assert D == HEAD_DIM and Hq % Hkv == 0

@@ -7,6 +7,8 @@ from typing import Optional
 
 import torch
 
+from . import _lib
+
 PAGE_SIZES = (32, 64, 128, 256)
 HEAD_DIM = 128
 FORMATS = ("bf16", "fp4")
@@ -27,6 +29,12 @@ class KVPages:
     v_scale: Optional[torch.Tensor] = None
 
     def __post_init__(self):
+        if self.k.is_cuda and (_lib._paged_host or _lib.paged_host()).pages_ok(self.k, self.v, self.k_scale, self.v_scale):
+            return
+        self.check()
+
+    def check(self):
+        """Raises ValueError where the tensors are not the pages of a layer."""
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
         if k.dim() != 4 or k.shape[2] not in PAGE_SIZES:
             raise ValueError(f"pages are (pages, heads, tokens, channels) with {PAGE_SIZES} tokens, got {tuple(k.shape)}")

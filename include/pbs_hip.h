@@ -269,7 +269,7 @@ int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale
  * 0 .. past_lens[b] + i; out (B, Hq, S, 128) with its own strides.  Rows from new_lens[b] on, and rows whose keys weigh nothing, are zeros.
  * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
  * positive.  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
-size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len);
+size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len);
 int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                        const int32_t* page_table, const int32_t* past_lens, const int32_t* new_lens, void* out, int B, int Hq, int Hkv,
                        int S, int head_dim, int num_pages, int max_pages, int page_size, int kv_bits, int max_len, int64_t q_sb,

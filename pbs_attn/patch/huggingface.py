@@ -6,6 +6,7 @@ from pbs_attn_amd.patch.huggingface import (  # noqa: F401
     get_flexprefill_prefill,
     get_meanpooling_prefill,
     get_minference_prefill,
+    get_paged_cache,
     get_permuted_block_sparse_attn_fwd,
     get_supported_model_types,
     get_xattention_prefill,

@@ -38,7 +38,7 @@ SIGNATURES = {
     "pbs_rope_qk": (c_int, [_P] * 6 + [_I] * 5 + [_L] * 8 + [_P]),
     "pbs_paged_append": (c_int, [_P] * 14 + [_I] * 9 + [_L] * 12 + [_P]),
     "pbs_paged_read": (c_int, [_P] * 8 + [_I] * 8 + [_L, _P]),
-    "pbs_paged_attn_workspace_bytes": (_Z, [_I] * 6),
+    "pbs_paged_attn_workspace_bytes": (_Z, [_I] * 7),
     "pbs_paged_attn_fwd": (c_int, [_P] * 9 + [_I] * 10 + [_L] * 7 + [_F, _P, _Z, _P]),
     "pbs_identity_indices": (c_int, [_P, _I, _I, _P]),
     "pbs_prefill_attn_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I]),

@@ -5,8 +5,7 @@
 #include <float.h>
 
 constexpr int PAGED_WAVES = 4;       // of a workgroup
-constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences: two a compute unit
-constexpr int PAGED_LEAST_STEPS = 2;   // steps that a worker takes at least
+constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences, at most: two a compute unit
 // A row's exponent is taken up where a logit is more than this above it (log2): weights stay below 2^8, which costs their sums in fp32 and their
 // roundings to bf16 nothing, and the sums are rescaled a few times in a sequence rather than with every new maximum.
 constexpr float PAGED_SLACK = 8.f;
@@ -23,7 +22,7 @@ struct PagedAttnArgs {
   const int32_t* fresh;   // null: S
   PagedHeader* headers;   // one a worker; null: a workgroup takes a whole row tile of one head
   float* parts;           // two slots a worker: the end of an earlier worker's piece, the beginning of the next one's
-  int B, Hq, Hkv, S, G, row_tiles;
+  int B, Hq, Hkv, S, G, row_tiles, workers;
   int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
   float scale_log2;   // softmax scale times log2(e)
 };
@@ -118,7 +117,7 @@ __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLd
     }
     total = __builtin_amdgcn_readfirstlane(total);
   }
-  const int share = max((int)(((unsigned)total + workers - 1) / workers), PAGED_LEAST_STEPS);
+  const int share = (int)(((unsigned)total + workers - 1) / workers);
   if ((int64_t)share * worker >= total) return false;
   const int start = share * worker;
   out->share = share;

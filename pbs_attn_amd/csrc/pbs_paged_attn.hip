@@ -6,6 +6,7 @@
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -13,7 +14,6 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
-constexpr int WAVES = PAGED_WAVES;
 constexpr int O_PITCH = PAGED_D + 4;
 
 // What a lane holds of a tile of 32 tokens.  n = lane % 16, g = lane / 16.
@@ -214,7 +214,7 @@ struct Softmax {
     for (int r = 0; r < R; ++r) {
       const int row = u.r0 + r * 16 + n, token = row / a.G;
       const bool valid = token < u.fresh;
-      if (R == 1 || wave == r % PAGED_WAVES) {
+      if (R == 1 || wave == r) {
         own.load(valid ? a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss : nullptr, g);
         if (R > 1) own.put(lds[r], g * 16 + n);
       }
@@ -302,8 +302,8 @@ struct Softmax {
   }
 };
 
-// Steps `s0` .. `s0 + steps - 1` of a unit and head, 4 * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
-template <int BITS, int R, int NT>
+// Steps `s0` .. `s0 + steps - 1` of a unit and head, WAVES * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
+template <int BITS, int R, int NT, int DEPTH, int WAVES>
 __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part,
                                      float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2], RowsLds* q_lds) {
   const int lane = paged_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -314,7 +314,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   const int end = min((s0 + steps) * WAVES * NT, tiles);
   // Loads go out DEPTH steps ahead, a step's K as soon as the K before it in the same registers has been multiplied, its V likewise.  Pages are
   // looked up before that; a tile that is not there is read as the pool's first one, and not used.
-  constexpr int DEPTH = NT == 2 ? 2 : 1, STRIDE = WAVES * NT;
+  constexpr int STRIDE = WAVES * NT;
   Tile<BITS> tile[DEPTH][NT];
   uint32_t gone[DEPTH] = {};
   int64_t at[NT];
@@ -408,6 +408,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     __syncthreads();
     // 16 lanes a row, 8 channels a lane
     const int rr = wave * 4 + g2, c = n2 * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
+    if (WAVES > 4 && wave >= 4) continue;
     float y[8], row_top = ml_lds[0][rr][0], sum = 0.f;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) row_top = fmaxf(row_top, ml_lds[w][rr][0]);
@@ -437,14 +438,14 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   __syncthreads();
 }
 
-template <int BITS, int R, int NT>
-__global__ __launch_bounds__(256, 2) void attn_kernel(PagedAttnArgs a) {
+template <int BITS, int R, int NT, int DEPTH, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_kernel(PagedAttnArgs a) {
   __shared__ float o_lds[WAVES][16][O_PITCH];
   __shared__ float ml_lds[WAVES][16][2];
   __shared__ PagedShareLds share_lds;
   __shared__ RowsLds q_lds[R > 1 ? R : 1];
   paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, false, [&](const PagedUnit& u, int head, int step, int steps, float* part)
-                                            __attribute__((always_inline)) { work<BITS, R, NT>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds); });
+                                            __attribute__((always_inline)) { work<BITS, R, NT, DEPTH, WAVES>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds); });
 }
 
 // Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it.  Sixteen lanes hold a
@@ -510,29 +511,36 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
 constexpr int step_of(int rows, int kv_bits) { return rows > 48 ? 64 : rows == 16 && kv_bits == 4 ? 256 : 128; }
 
 struct Plan {
-  int rows;   // of a row tile
-  bool cut;
+  int rows;      // of a row tile
+  int workers;   // 0: sequences are not cut
   size_t bytes;
 };
-Plan plan_of(int B, int Hq, int Hkv, int S, int max_len) {
+Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : rows <= 64 ? 64 : 128;
-  p.cut = max_len > 512 && (p.rows <= 48 || B * ((rows + p.rows - 1) / p.rows) * Hkv < 4 * PAGED_WORKERS);
-  p.bytes = p.cut ? PAGED_WORKERS * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows)) : 0;
+  // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512
+  // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.
+  const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
+  const bool cut = max_len > (kv_bits == 16 ? 640 : 1280) && (p.rows <= 48 || units < 4 * PAGED_WORKERS);
+  // (no more workers than there is work for)
+  const int64_t steps = units * ((max_len + step_of(p.rows, kv_bits) - 1) / step_of(p.rows, kv_bits));
+  p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS, steps + 7) / 8 * 8 : 0;
+  p.bytes = p.workers * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows));
   return p;
 }
 
 template <int BITS, int R, int NT>
 void launch(const PagedAttnArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((attn_kernel<BITS, R, NT>), dim3(a.headers ? PAGED_WORKERS : a.Hkv * a.B * a.row_tiles), dim3(256), 0, stream, a);
+  if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, NT, 4>), dim3(a.workers), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((attn_kernel<BITS, R, NT, NT, 8>), dim3(a.Hkv * a.B * a.row_tiles), dim3(512), 0, stream, a);
 }
 
 }  // namespace
 
-extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int max_len) {
+extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || S <= 0 || Hq < Hkv || max_len <= 0) return 0;
-  return plan_of(B, Hq, Hkv, S, max_len).bytes;
+  return plan_of(B, Hq, Hkv, S, kv_bits, max_len).bytes;
 }
 
 extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
@@ -551,7 +559,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   PBS_REQUIRE(softmax_scale > 0.f && softmax_scale <= FLT_MAX, "pbs_paged_attn_fwd: softmax_scale must be positive and finite");
   PBS_REQUIRE(((q_sb | q_sh | q_ss | o_sb | o_sh | o_ss) % 8) == 0, "pbs_paged_attn_fwd: strides must keep rows 16-byte aligned");
   PBS_REQUIRE((((uintptr_t)q | (uintptr_t)out) % 16) == 0, "pbs_paged_attn_fwd: pointers must be 16-byte aligned");
-  Plan p = plan_of(B, Hq, Hkv, S, max_len);
+  Plan p = plan_of(B, Hq, Hkv, S, kv_bits, max_len);
   PBS_REQUIRE(p.bytes == 0 || (workspace && ((uintptr_t)workspace % 256) == 0 && workspace_bytes >= p.bytes),
               "pbs_paged_attn_fwd: workspace of %zu bytes, 256-byte aligned, needed", p.bytes);
   a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.past = past_lens; a.fresh = new_lens;
@@ -561,10 +569,11 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.row_tiles = (S * a.G + p.rows - 1) / p.rows;
   const int64_t units = (int64_t)B * Hkv * a.row_tiles;
   PBS_REQUIRE(units < (1 << 24), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
-  // the line of steps that workers share has to fit 32 bits, whatever the lengths are (units of two thirds of a million keys each fill the chip)
-  if (units * (((int64_t)max_pages * page_size + 63) / step_of(p.rows, kv_bits) + 1) > INT32_MAX) p.cut = false;
-  a.headers = p.cut ? (PagedHeader*)workspace : nullptr;
-  a.parts = p.cut ? (float*)((char*)workspace + PAGED_WORKERS * sizeof(PagedHeader)) : nullptr;
+  // the line of steps that workers share has to fit 32 bits, whatever the lengths turn out to be: a call that may not is not cut
+  if (units * ((int64_t)max_pages * page_size / step_of(p.rows, kv_bits) + 1) > INT32_MAX) p.workers = 0;
+  a.workers = p.workers;
+  a.headers = p.workers ? (PagedHeader*)workspace : nullptr;
+  a.parts = p.workers ? (float*)((char*)workspace + p.workers * sizeof(PagedHeader)) : nullptr;
   hipStream_t st = (hipStream_t)stream;
   if (p.rows > 48) {
     if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
@@ -577,10 +586,11 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
     else if (p.rows == 32) launch<4, 2, 1>(a, st);
     else launch<4, 3, 1>(a, st);
   }
-  if (p.cut) {
-    if (p.rows == 16) hipLaunchKernelGGL(join_kernel<16>, dim3(PAGED_WORKERS, p.rows), dim3(256), 0, st, a, p.rows);
-    else if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<4>, dim3(PAGED_WORKERS, p.rows / 4), dim3(256), 0, st, a, p.rows);
-    else hipLaunchKernelGGL(join_kernel<1>, dim3(PAGED_WORKERS, p.rows / 16), dim3(256), 0, st, a, p.rows);
+  if (p.workers) {
+    const int rows = (int)std::min<int64_t>(p.rows, (int64_t)S * a.G);
+    if (p.rows == 16) hipLaunchKernelGGL(join_kernel<16>, dim3(p.workers, rows), dim3(256), 0, st, a, p.rows);
+    else if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<4>, dim3(p.workers, (rows + 3) / 4), dim3(256), 0, st, a, p.rows);
+    else hipLaunchKernelGGL(join_kernel<1>, dim3(p.workers, (rows + 15) / 16), dim3(256), 0, st, a, p.rows);
   }
   return pbs_check_launch("pbs_paged_attn_fwd");
 }

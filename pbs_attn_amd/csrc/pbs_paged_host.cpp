@@ -196,7 +196,7 @@ PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (max_len <= 0) return not_taken();
   void* stream;
   if (!stream_of(*q, &stream)) return not_taken();
-  const size_t bytes = attn_bytes_fn((int)B, (int)Hq, (int)pages.heads, (int)S, HEAD_DIM, (int)max_len);
+  const size_t bytes = attn_bytes_fn((int)B, (int)Hq, (int)pages.heads, (int)S, HEAD_DIM, pages.bits(), (int)max_len);
   at::Tensor out = at::empty({B, Hq, S, HEAD_DIM}, q->options()), ws;
   if (bytes) ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
   int rc;

@@ -305,7 +305,7 @@ int launch(const PagedAttnArgs& a, hipStream_t stream) {
     pbs_set_error("pbs_paged_attn_fwd: hipFuncSetAttribute: %s", hipGetErrorString(e));
     return (int)e;
   }
-  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), dim3(a.headers ? PAGED_WORKERS : a.Hkv * a.B * a.row_tiles), dim3(256), LDS_TOTAL, stream, a);
+  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), dim3(a.headers ? a.workers : a.Hkv * a.B * a.row_tiles), dim3(256), LDS_TOTAL, stream, a);
   return 0;
 }
 

@@ -507,7 +507,7 @@ def paged_attn(q, pages, page_table, past_lens, new_lens=None, softmax_scale=Non
     q, q_ptr, q_strides = _rows16_args(q)
     out = q.new_empty(B, Hq, S, D)
     lib = _lib.load()
-    ws_bytes = lib.pbs_paged_attn_workspace_bytes(B, Hq, Hkv, S, D, max_len)
+    ws_bytes = lib.pbs_paged_attn_workspace_bytes(B, Hq, Hkv, S, D, bits, max_len)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     with _on_device_of(q):
         rc = lib.pbs_paged_attn_fwd(

@@ -13,6 +13,9 @@ Two extensions: a prefill function whose underlying python function carries
 ``repeat_kv`` copies (the PBS HIP path reads KV head h // group itself); and bf16
 head-dim-128 prompts on the GPU get their rotary embedding from one HIP kernel
 that produces the same bits as the tensor expression.
+
+With a paged cache (``get_paged_cache``) as ``past_key_values`` a layer's keys and values go into its pages, and single tokens and later prompts
+attend to them.
 """
 from __future__ import annotations
 
@@ -115,6 +118,15 @@ def get_permuted_block_sparse_attn_fwd(
     return partial(impl, **settings)
 
 
+def get_paged_cache(model, batch_size, max_len, page_size=64, form="bf16"):
+    """A ``PagedKVCache`` (pbs_attn_amd/patch/paged_cache.py) for a model whose layers are patched: pass it as ``past_key_values``.  ``form``:
+    "bf16", or "fp4" for 4 bits."""
+    from pbs_attn_amd.patch.paged_cache import PagedKVCache
+    k_proj = model.model.layers[0].self_attn.k_proj
+    head_dim = getattr(model.config, "head_dim", None) or model.config.hidden_size // model.config.num_attention_heads
+    return PagedKVCache(model.config, batch_size, max_len, page_size, form, k_proj.weight.device, k_proj.weight.shape[0] // head_dim)
+
+
 def _underlying(fn):
     return fn.func if isinstance(fn, partial) else fn
 
@@ -133,6 +145,11 @@ def _fused_rope_applies(q, k, cos, sin):
             and cos.stride() == sin.stride())
 
 
+def _paged_layer(cache, layer_idx):
+    """The layer of a paged cache, None for any other cache."""
+    return cache.layers[layer_idx] if getattr(cache, "is_paged", False) else None
+
+
 def patched_attention_forward(
     self,
     hidden_states: torch.Tensor,
@@ -145,7 +162,8 @@ def patched_attention_forward(
 ):
     """Replacement for ``LlamaAttention.forward`` / ``Qwen2Attention.forward``."""
     bsz, q_len, _ = hidden_states.size()
-    if q_len <= 1:
+    pages = _paged_layer(past_key_values, self.layer_idx)
+    if q_len <= 1 and pages is None:
         return self.original_forward(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                      attention_mask=attention_mask, past_key_values=past_key_values,
                                      cache_position=cache_position, **kwargs)
@@ -155,17 +173,24 @@ def patched_attention_forward(
     v, _ = _split_heads(self.v_proj(hidden_states), bsz, q_len, self.head_dim)
 
     cos, sin = position_embeddings
-    if _fused_rope_applies(q, k, cos, sin):
+    if pages is not None and (q_len == 1 or pages.length > 0):
+        # on a filled cache, or one token: rotated into the pages, which hold all that the queries see
+        q, _ = pages.append(k, v, q=q, cos=cos, sin=sin)
+        attn = pages.attention(q).transpose(1, 2).reshape(bsz, q_len, n_q * self.head_dim)
+        return self.o_proj(attn), None
+    if prefill_fn is None:
+        raise RuntimeError("prefill_fn required.")
+    if pages is not None:
+        q, k = pages.append(k, v, q=q, cos=cos, sin=sin, want_k=True)
+    elif _fused_rope_applies(q, k, cos, sin):
         # same bits as apply_rotary_pos_emb, one kernel instead of ten, head-major contiguous outputs
         from pbs_attn_amd import ops
         q, k = ops.rope_qk(q, k, cos, sin)
     else:
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
-    if past_key_values is not None:
+    if past_key_values is not None and pages is None:
         past_key_values.update(k, v, self.layer_idx, {"sin": sin, "cos": cos, "cache_position": cache_position})
 
-    if prefill_fn is None:
-        raise RuntimeError("prefill_fn required.")
     kernel_fn = _underlying(prefill_fn)
     if not getattr(kernel_fn, "native_gqa", False):
         n_rep = max(1, n_q // max(1, n_kv))

@@ -1,0 +1,96 @@
+"""A paged key-value cache for patched Hugging Face models: ``model(ids, past_key_values=PagedKVCache(...))``, ``model.generate(...)``.
+
+A patched layer (``apply_patch_with_prefill``) that is handed this cache writes its keys and values into the pages with the rotary embedding
+on the way.  The first prompt's attention is the prefill function's; single tokens and later prompts attend to the pages
+(``ops.paged_attn``), where the reference sends single tokens to the module's original forward and lets a later prompt attend to itself
+alone (pbs_attn/patch/huggingface.py:169-241).  Layers that are not patched (``skip_layers``) read their keys and values back (``update``).
+
+All sequences of a batch have one length, as the module's inputs have: there is no padding, and attention masks are not looked at (the
+prefill function takes none either).  The lengths are the host's: a program that captures its decoding step into a graph calls
+``ops.paged_append`` and ``ops.paged_attn`` with lengths of its own on the GPU."""
+from __future__ import annotations
+
+import torch
+from transformers.cache_utils import Cache, CacheLayerMixin
+
+from pbs_attn_amd import ops
+from pbs_attn_amd.paged import HEAD_DIM, PAGE_SIZES, alloc_pages
+
+
+class _PagedLayer(CacheLayerMixin):
+    def __init__(self, cache, pages):
+        super().__init__()
+        self.cache, self.pages, self.length = cache, pages, 0
+        self.is_initialized = True
+
+    def lazy_initialization(self, key_states, value_states):
+        pass
+
+    def append(self, k, v, **rotation):
+        """New tokens k, v (batch, heads, S, 128) behind those that are there; the arguments and results of ``ops.paged_append``."""
+        if k.shape[0] != self.cache.sequences:
+            raise ValueError(f"a cache of {self.cache.sequences} sequences, {k.shape[0]} given")
+        if self.length + k.shape[2] > self.cache.room:
+            raise ValueError(f"{self.length} + {k.shape[2]} tokens, and the cache holds {self.cache.room}")
+        rotated = ops.paged_append(self.pages, self.cache.page_table, self.cache.lengths(self.length), k, v, **rotation)
+        self.length += k.shape[2]
+        return rotated
+
+    def attention(self, q):
+        """Of the last tokens, appended before: q (batch, heads, S, 128)."""
+        past = self.length - q.shape[2]
+        return ops.paged_attn(q, self.pages, self.cache.page_table, self.cache.lengths(past), max_len=self.length)
+
+    def update(self, key_states, value_states, *args, **kwargs):
+        """For modules with an attention of their own: stores the (rotated) keys and the values, and returns all of them."""
+        self.append(key_states, value_states)
+        return ops.paged_read(self.pages, self.cache.page_table, self.cache.lengths(self.length), self.length)
+
+    def get_mask_sizes(self, query_length, *args):
+        return self.length + query_length, 0
+
+    def get_seq_length(self, *args):
+        return self.length
+
+    def get_max_length(self):
+        return self.cache.room
+
+    get_max_cache_shape = get_max_length
+
+    def reset(self):
+        self.length = 0
+
+    def reorder_cache(self, beam_idx):
+        raise NotImplementedError("a paged cache does not reorder its sequences")
+
+
+class PagedKVCache(Cache):
+    """Room for ``batch_size`` sequences of up to ``max_len`` tokens of a model with ``config``, in pages of ``page_size`` tokens, bf16 or
+    4 bits (``form="fp4"``: about a quarter of the memory and of a decoding step's traffic; the first prompt's own attention still sees bf16).
+    ``num_kv_heads``: of this process, where it is not the configuration's (tensor parallel)."""
+
+    is_paged = True
+
+    def __init__(self, config, batch_size, max_len, page_size=64, form="bf16", device="cuda", num_kv_heads=None):
+        head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+        if head_dim != HEAD_DIM:
+            raise ValueError(f"a paged cache holds heads of {HEAD_DIM}, not {head_dim}")
+        if batch_size <= 0 or max_len <= 0:
+            raise ValueError("a cache holds at least one sequence of at least one token")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"pages of {PAGE_SIZES} tokens, got {page_size}")
+        heads = num_kv_heads or config.num_key_value_heads
+        slots = (max_len + page_size - 1) // page_size
+        self.sequences, self.room = batch_size, max_len
+        self.page_table = torch.arange(batch_size * slots, dtype=torch.int32, device=device).view(batch_size, slots)
+        self._lengths = {}
+        super().__init__(layers=[_PagedLayer(self, alloc_pages(batch_size * slots, heads, page_size, form, device))
+                                 for _ in range(config.num_hidden_layers)])
+
+    def lengths(self, n):
+        """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same."""
+        if n not in self._lengths:
+            if len(self._lengths) >= 2:
+                del self._lengths[next(iter(self._lengths))]
+            self._lengths[n] = torch.full((self.sequences,), n, dtype=torch.int32, device=self.page_table.device)
+        return self._lengths[n]

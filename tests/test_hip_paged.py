@@ -338,3 +338,52 @@ def test_a_captured_decoding_step(dev, form):
             want, tol = attention(q_rot[b], kk, vv, n, 1, 128 ** -0.5)
             assert ((got[b].double() - want).abs() <= tol).all(), (i, b)
         past += 1
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_calls_without_the_native_module_give_the_same_bits(dev, form, monkeypatch):
+    from pbs_attn_amd import _lib
+    f = Filled(form, 8, 2, 3, [700, 64], page=64)
+    assert _lib.paged_host() is not _lib._no_paged_host
+    want, read = f.attn(softmax_scale=0.1, max_len=703), ops.paged_read(f.pages, f.table, f.past, 700)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, q, cos = _randn(g, 2, 2, 3, 128), _randn(g, 2, 8, 3, 128), _randn(g, 1, 3, 128)
+    rotated_natively = ops.paged_append(f.pages, f.table, f.past, k, k, q=q, cos=cos, sin=cos, want_k=True)
+    stored = ops.paged_read(f.pages, f.table, f.past + 3, 703)
+    monkeypatch.setattr(_lib, "_paged_host", _lib._no_paged_host)
+    again = ops.paged_append(f.pages, f.table, f.past, k, k, q=q, cos=cos, sin=cos, want_k=True)
+    assert all(torch.equal(a, b) for a, b in zip(again, rotated_natively))
+    assert all(torch.equal(a.nan_to_num(9), b.nan_to_num(9)) for a, b in zip(ops.paged_read(f.pages, f.table, f.past + 3, 703), stored))
+    f2 = Filled(form, 8, 2, 3, [700, 64], page=64)
+    assert torch.equal(f2.attn(softmax_scale=0.1, max_len=703), want)
+    assert all(torch.equal(a, b) for a, b in zip(ops.paged_read(f2.pages, f2.table, f2.past, 700), read))
+
+
+def test_native_calls_refuse_what_the_general_path_refuses(dev):
+    """The same messages, as the native call hands over what is not plain."""
+    f = Filled("bf16", 8, 2, 1, [70], page=64)
+    k = torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="pages of 2 heads"):
+        ops.paged_append(f.pages, f.table, f.past, k[:, :1], k[:, :1])
+    with pytest.raises(ValueError, match="page_table"):
+        ops.paged_attn(f.q, f.pages, f.table.long(), f.past)
+    with pytest.raises(ValueError, match="lengths"):
+        ops.paged_attn(f.q, f.pages, f.table, f.past.long())
+    with pytest.raises(ValueError, match="lengths"):
+        ops.paged_read(f.pages, f.table, f.past.cpu().repeat(2), 5)
+    with pytest.raises(ValueError, match="tensors on cpu"):
+        ops.paged_read(f.pages, f.table, f.past.cpu(), 5)
+    with pytest.raises(ValueError, match="max_len"):
+        ops.paged_read(f.pages, f.table, f.past, 0)
+    from pbs_attn_amd._lib import PbsHipError
+    with pytest.raises(PbsHipError, match="softmax_scale"):
+        ops.paged_attn(f.q, f.pages, f.table, f.past, softmax_scale=-1.0)
+    with pytest.raises(PbsHipError, match="max_len"):
+        ops.paged_attn(f.q, f.pages, f.table, f.past, max_len=0)
+    with pytest.raises(PbsHipError, match="bf16 only"):
+        ops.paged_attn(f.q.float(), f.pages, f.table, f.past)
+    with pytest.raises(AssertionError):
+        ops.paged_attn(f.q[:, :7], f.pages, f.table, f.past)
+    f.pages.v = f.pages.v[:1]
+    with pytest.raises(ValueError, match="pages are either"):
+        ops.paged_attn(f.q, f.pages, f.table, f.past)

@@ -91,3 +91,62 @@ def test_there_is_no_cpu_path():
         ops.paged_attn(x[..., :64], p, table, n)
     with pytest.raises(ValueError, match="cos goes with sin"):
         ops.paged_append(p, table, n, x, x, cos=x[0])
+
+
+def _config(**kw):
+    from transformers import LlamaConfig
+    return LlamaConfig(**{**dict(hidden_size=512, num_attention_heads=4, num_key_value_heads=2, head_dim=128, num_hidden_layers=3), **kw})
+
+
+def test_paged_cache_of_a_model():
+    from pbs_attn_amd.patch.paged_cache import PagedKVCache
+    cache = PagedKVCache(_config(), 2, 100, page_size=32, device="cpu")
+    assert cache.page_table.shape == (2, 4) and len(cache.layers) == 3 and cache.layers[1].pages.k.shape == (8, 2, 32, 128)
+    assert cache.get_seq_length() == 0 and cache.layers[2].get_mask_sizes(5) == (5, 0) and cache.layers[0].get_max_length() == 100
+    assert cache.lengths(3) is cache.lengths(3) and cache.lengths(3).tolist() == [3, 3]
+    cache.lengths(4), cache.lengths(5)
+    assert len(cache._lengths) == 2 and cache.lengths(3).tolist() == [3, 3]
+    assert PagedKVCache(_config(), 1, 100, form="fp4", device="cpu", num_kv_heads=1).layers[0].pages.k.shape == (2, 1, 64, 64)
+    with pytest.raises(ValueError, match="2 sequences"):
+        cache.layers[0].append(torch.zeros(1, 2, 1, 128), torch.zeros(1, 2, 1, 128))
+    with pytest.raises(ValueError, match="the cache holds 100"):
+        cache.layers[0].append(torch.zeros(2, 2, 101, 128), torch.zeros(2, 2, 101, 128))
+    x = torch.zeros(2, 2, 1, 128, dtype=torch.bfloat16)
+    with pytest.raises(_lib.PbsHipError, match="GPU"):
+        cache.update(x, x, 0)
+    assert cache.get_seq_length() == 0     # nothing was stored
+    with pytest.raises(NotImplementedError):
+        cache.reorder_cache(torch.zeros(2, dtype=torch.long))
+    for bad in [dict(config=_config(head_dim=64)), dict(batch_size=0), dict(max_len=0), dict(page_size=48), dict(form="int4")]:
+        with pytest.raises(ValueError):
+            PagedKVCache(**{**dict(config=_config(), batch_size=1, max_len=8, device="cpu"), **bad})
+
+
+@pytest.mark.parametrize("kind", ["missing", "of another kind"])
+def test_without_the_native_module_python_takes_every_call(kind, monkeypatch, tmp_path):
+    path = tmp_path / "module.so"
+    if kind != "missing":
+        path.write_bytes(b"no module")
+    monkeypatch.setattr(_lib, "PAGED_HOST_PATH", str(path))
+    monkeypatch.setattr(_lib, "_paged_host", None)
+    with pytest.warns(UserWarning, match="through Python"):
+        host = _lib.paged_host()
+    assert host.append() is None and host.attn() is None and host.read() is None and host.pages_ok() is None and _lib.paged_host() is host
+
+
+def test_the_native_module_takes_plain_calls_only():
+    import os
+    if not os.path.exists(_lib.PAGED_HOST_PATH):
+        from pbs_attn_amd.build import build_paged_host_module
+        build_paged_host_module()
+    host = _lib.paged_host()
+    assert host is not _lib._no_paged_host
+    p = alloc_pages(3, 2, 64, "bf16", "cpu")
+    x, table, n = torch.zeros(1, 2, 4, 128, dtype=torch.bfloat16), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    assert host.pages_ok(p.k, p.v, None, None) is False            # (not on the GPU)
+    assert host.append(p, table, n, x, x, None, None, None, None, False) is None
+    assert host.attn(x, p, table, n, None, None, None) is None and host.read(p, table, n, 5) is None
+    assert host.append(*[None] * 10) is None and host.attn(*"abcdefg") is None and host.read(1, 2.0, "3", 4) is None
+    for call in (host.append, host.attn, host.read, host.pages_ok):
+        with pytest.raises(TypeError):
+            call(p)

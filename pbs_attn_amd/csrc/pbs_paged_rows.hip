@@ -5,6 +5,7 @@
 // during the tile before and unpacked to bf16 behind it, once for all rows.
 #include "pbs_paged_attn.h"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -163,8 +164,10 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     stage.store(buffer, held0, held1);
   }
   for (int step = s0; step < end; ++step) {
-    // this tile's copies have landed, and nobody reads the other buffer any more
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // this tile's copies have landed, and nobody reads the other buffer any more.  (By the builtin: the compiler sees that the queries have
+    // landed too, and does not wait for them behind the next copies, which it does not count.)
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    asm volatile("" ::: "memory");
     __syncthreads();
     if (step + 1 < end) {
       look_up(step + 1, at0, at1, next0, next1);
@@ -238,20 +241,24 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         }
       l[r] += sum;
     }
+    auto add = [&](auto tail) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        u32x4 x = *(const u32x4*)(vt + ((4 * i + g) * PAGED_D + d * 16 + n) * 16);
-        if (BITS == 16 && !whole) {   // tokens that are not there hold whatever the page held before: not even times zero
-          const int held = (i ? held1 : held0) - 8 * g;
+        for (int d = 0; d < 8; ++d) {
+          u32x4 x = *(const u32x4*)(vt + ((4 * i + g) * PAGED_D + d * 16 + n) * 16);
+          if (tail.value) {   // tokens that are not there hold whatever the page held before: not even times zero
+            const int held = (i ? held1 : held0) - 8 * g;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) x[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
+            for (int w = 0; w < 4; ++w) x[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
+          }
+          const bf16x8 v = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+          for (int r = 0; r < RW; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][i], o[r][d], 0, 0, 0);
         }
-        const bf16x8 v = __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-        for (int r = 0; r < RW; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][i], o[r][d], 0, 0, 0);
-      }
+    };
+    if (BITS == 4 || held0 + held1 == KEYS) add(std::false_type{});
+    else add(std::true_type{});
     held0 = next0;
     held1 = next1;
     buffer ^= LDS_BUFFER;

@@ -5,7 +5,6 @@
 // during the tile before and unpacked to bf16 behind it, once for all rows.
 #include "pbs_paged_attn.h"
 #include <math.h>
-#include <type_traits>
 
 namespace {
 
@@ -173,26 +172,50 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       look_up(step + 1, at0, at1, next0, next1);
       stage.load(a.pool, at0, at1, buffer ^ LDS_BUFFER, wave, lane);
     }
+    if (BITS == 16 && held0 + held1 < KEYS) {
+      // tokens that are not there hold whatever the page held before: not even times zero
+      for (int i = threadIdx.x; i < KEYS / 8 * PAGED_D; i += 256) {
+        const int held = (i < 4 * PAGED_D ? held0 : held1) - (i / PAGED_D & 3) * 8;
+        u32x4* x = (u32x4*)(lds + buffer + LDS_V) + i;
+        if (held < 8) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) (*x)[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
+        }
+      }
+      __syncthreads();
+    }
     const int k0 = step * KEYS;
     const bool whole = k0 + KEYS <= u.all_see && held0 + held1 == KEYS;
     const char* kt = lds + buffer;
     const char* vt = lds + buffer + LDS_V;
+    // Operands are read from LDS two groups of four ahead of the products that take them; the fences keep the compiler from sinking the reads.
     f32x4 s[RW][2][2];
+    bf16x8 k[3][4], v[3][4];
+    auto read_k = [&](int i) __attribute__((always_inline)) {
+      // operand row n is token 32 (i / 2) + 2 n + i % 2: a lane ends up with the logits of eight tokens in a row, 32 (i / 2) + 8 g ..
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int e = 0; e < 4; ++e) k[i % 3][e] = *(const bf16x8*)(kt + k_place(32 * (i >> 1) + 2 * n + (i & 1), e * 4 + g));
+    };
+    auto read_v = [&](int i) __attribute__((always_inline)) {   // channels 16 d + n, d = 4 (i % 2) .., of tokens 32 (i / 2) + 8 g ..
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // operand row n is token 32 i + 2 n + h: a lane ends up with the logits of eight tokens in a row, 32 i + 8 g ..
-        bf16x8 k[4];
+      for (int e = 0; e < 4; ++e) v[i % 3][e] = *(const bf16x8*)(vt + ((4 * (i >> 1) + g) * PAGED_D + (4 * (i & 1) + e) * 16 + n) * 16);
+    };
+    auto fence = [] __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    read_k(0);
+    read_k(1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = *(const bf16x8*)(kt + k_place(32 * i + 2 * n + h, e * 4 + g));
+    for (int i = 0; i < 4; ++i) {
+      fence();
+      if (i < 2) read_k(i + 2);
+      else read_v(i - 2);
 #pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          s[r][i][h] = (f32x4){};
+      for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = (f32x4){};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[r][i][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[e], q[r][e], s[r][i][h], 0, 0, 0);
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % 3][e], q[r][e], s[r][i >> 1][i & 1], 0, 0, 0);
+    }
+    fence();
     if (!whole) {
 #pragma unroll
       for (int r = 0; r < RW; ++r)
@@ -228,37 +251,31 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         m[r] = m_new;
       }
     }
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
+    auto weigh = [&](int r, int i) __attribute__((always_inline)) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
-          sum += e;
-          p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
+        sum += e;
+        p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
+      }
       l[r] += sum;
-    }
-    auto add = [&](auto tail) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          u32x4 x = *(const u32x4*)(vt + ((4 * i + g) * PAGED_D + d * 16 + n) * 16);
-          if (tail.value) {   // tokens that are not there hold whatever the page held before: not even times zero
-            const int held = (i ? held1 : held0) - 8 * g;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) x[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
-          }
-          const bf16x8 v = __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-          for (int r = 0; r < RW; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][i], o[r][d], 0, 0, 0);
-        }
     };
-    if (BITS == 4 || held0 + held1 == KEYS) add(std::false_type{});
-    else add(std::true_type{});
+    // weights of the first 32 keys; then their products, and beside them the weights of the other 32
+#pragma unroll
+    for (int r = 0; r < RW; ++r) weigh(r, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fence();
+      if (i < 2) read_v(i + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < RW; ++r)
+          o[r][4 * (i & 1) + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i % 3][e], p[r][i >> 1], o[r][4 * (i & 1) + e], 0, 0, 0);
+      if (i < RW) weigh(i, 1);
+    }
+    fence();
     held0 = next0;
     held1 = next1;
     buffer ^= LDS_BUFFER;

@@ -36,12 +36,6 @@ __device__ __forceinline__ float max_over_groups(float v) {   // lanes l, l ^ 16
   t = with_lane_xor<32>(__float_as_uint(v));
   return fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
 }
-__device__ __forceinline__ float sum_over_groups(float v) {
-  TwoOf t = with_lane_xor<16>(__float_as_uint(v));
-  v = __uint_as_float(t.a) + __uint_as_float(t.b);
-  t = with_lane_xor<32>(__float_as_uint(v));
-  return __uint_as_float(t.a) + __uint_as_float(t.b);
-}
 
 // lane id formed where it is asked for: what is derived from it holds no registers elsewhere
 __device__ __forceinline__ int paged_lane() {

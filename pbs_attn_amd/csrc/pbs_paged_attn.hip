@@ -205,7 +205,8 @@ struct Softmax {
   Rows<BITS> own;
   RowsLds* lds;
   f32x4 o[R][8];
-  float m[R], l[R];
+  float m[R];
+  f32x4 l[R];   // the weights' sums, as products with ones (every row of the tile the same): 32 bits, on the matrix unit, and no sum over lanes
   int seen[R];
 
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedUnit& u, int head, int n, int g, int wave, RowsLds* q_lds) {
@@ -220,7 +221,7 @@ struct Softmax {
       }
       seen[r] = valid ? u.past + token + 1 : 0;
       m[r] = -FLT_MAX;
-      l[r] = 0.f;
+      l[r] = (f32x4){};
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[r][d] = (f32x4){};
     }
@@ -256,32 +257,30 @@ struct Softmax {
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], x[r][i][j]);
-      top[r] = max_over_groups(top[r]) * c;
-      grows |= top[r] > m[r] + PAGED_SLACK;
+      grows |= top[r] * c > m[r] + PAGED_SLACK;   // (this lane's keys; the row's are looked at where one of them is)
     }
     if (__any(grows)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float m_new = fmaxf(m[r], top[r]), f = __builtin_amdgcn_exp2f(m[r] - m_new);
+        const float m_new = fmaxf(m[r], max_over_groups(top[r]) * c), f = __builtin_amdgcn_exp2f(m[r] - m_new);
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;
         m[r] = m_new;
       }
     }
+    bf16x8 ones;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float sum = 0.f;
+    for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.f;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i][j], c, -m[r]));
-          sum += e;
-          p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
-        }
-      l[r] += sum;
-    }
+      for (int i = 0; i < NT; ++i) {
+        // half a step of 2^-8 off, above the line and below it
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i][j], c, -m[r]));
+        l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i], l[r], 0, 0, 0);
+      }
   }
   template <bool TAIL>
   __device__ __forceinline__ void add(const Tile<BITS> (&t)[NT], const bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, int g) {
@@ -390,7 +389,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   const int lane2 = paged_lane(), n2 = lane2 & 15, g2 = lane2 >> 4;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float l = sum_over_groups(s.l[r]);
+    const float l = s.l[r][0];
     if (r > 0) __syncthreads();   // (the rows before have been read)
     if (g2 == 0) {
       ml_lds[wave][n2][0] = s.m[r];

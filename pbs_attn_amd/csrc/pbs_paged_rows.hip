@@ -122,7 +122,8 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   const float c = a.scale_log2;
   bf16x8 q[RW][4];
   f32x4 o[RW][8];
-  float m[RW], l[RW];
+  float m[RW];
+  f32x4 l[RW];   // the weights' sums, as products with ones (every row of the tile the same): 32 bits, on the matrix unit, and no sum over lanes
   int seen[RW];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -137,11 +138,14 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     }
     seen[r] = valid ? u.past + token + 1 : 0;
     m[r] = -FLT_MAX;
-    l[r] = 0.f;
+    l[r] = (f32x4){};
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[r][d] = (f32x4){};
   }
   const int end = min(s0 + steps, (u.keys + KEYS - 1) / KEYS);
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.f;
   Stage<BITS> stage;
   stage.begin(wave, lane);
   // tiles of a step: where they are, and how many of their 32 keys (0 where the page is not there)
@@ -238,13 +242,12 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], s[r][i][j & 1][j >> 1]);
-      top[r] = max_over_groups(top[r]) * c;
-      grows |= top[r] > m[r] + PAGED_SLACK;
+      grows |= top[r] * c > m[r] + PAGED_SLACK;   // (this lane's keys; the row's are looked at where one of them is)
     }
     if (__any(grows)) {
 #pragma unroll
       for (int r = 0; r < RW; ++r) {
-        const float m_new = fmaxf(m[r], top[r]), f = __builtin_amdgcn_exp2f(m[r] - m_new);
+        const float m_new = fmaxf(m[r], max_over_groups(top[r]) * c), f = __builtin_amdgcn_exp2f(m[r] - m_new);
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;
@@ -252,14 +255,9 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       }
     }
     auto weigh = [&](int r, int i) __attribute__((always_inline)) {
-      float sum = 0.f;
+      // half a step of 2^-8 off, above the line and below it
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
-        sum += e;
-        p[r][i][j] = (__bf16)e;   // (half a step of 2^-8 off: weights are summed as they are, and multiply bf16 values)
-      }
-      l[r] += sum;
+      for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
     };
     // weights of the first 32 keys; then their products, and beside them the weights of the other 32
 #pragma unroll
@@ -274,6 +272,10 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         for (int r = 0; r < RW; ++r)
           o[r][4 * (i & 1) + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i % 3][e], p[r][i >> 1], o[r][4 * (i & 1) + e], 0, 0, 0);
       if (i < RW) weigh(i, 1);
+      if (i & 1) {
+#pragma unroll
+        for (int r = 0; r < RW; ++r) l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i >> 1], l[r], 0, 0, 0);
+      }
     }
     fence();
     held0 = next0;
@@ -284,7 +286,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
-    const float sum = sum_over_groups(l[r]);
+    const float sum = l[r][0];
     const int rr = (wave * RW + r) * 16 + n, row = u.r0 + rr, token = row / a.G;
     if (part) {
 #pragma unroll

@@ -275,7 +275,7 @@ extern "C" int pbs_paged_read(const void* k_pages, const void* v_pages, const vo
                                 max_pages, page_size, kv_bits))
     return rc;
   PBS_REQUIRE(lens && k_out && v_out, "pbs_paged_read: null tensor pointer");
-  PBS_REQUIRE(max_len > 0, "pbs_paged_read: bad shape");
+  PBS_REQUIRE(max_len > 0 && max_len <= (1 << 28), "pbs_paged_read: bad shape");   // (a grid's threads fit 32 bits)
   PBS_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) % 16) == 0, "pbs_paged_read: pointers must be 16-byte aligned");
   a.lens = lens; a.k_out = (uint16_t*)k_out; a.v_out = (uint16_t*)v_out; a.L = max_len;
   const dim3 grid((max_len + PAGED_TILE - 1) / PAGED_TILE, Hkv, B);

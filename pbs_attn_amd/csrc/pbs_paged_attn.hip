@@ -403,7 +403,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
     for (int d = 0; d < 8; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = f == 0.f ? 0.f : s.o[r][d][i] * f;
+      for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = s.o[r][d][i] * f;
     __syncthreads();
     // 16 lanes a row, 8 channels a lane
     const int rr = wave * 4 + g2, c = n2 * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
@@ -472,8 +472,8 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
       const float m = fmaxf(top, ml.x), old = __builtin_amdgcn_exp2f(top - m), now = __builtin_amdgcn_exp2f(ml.x - m);
       top = m;
       sum = sum * old + ml.y * now;
-      y0 = (old == 0.f ? (f32x4){} : y0 * old) + (now == 0.f ? (f32x4){} : x0 * now);
-      y1 = (old == 0.f ? (f32x4){} : y1 * old) + (now == 0.f ? (f32x4){} : x1 * now);
+      y0 = y0 * old + x0 * now;
+      y1 = y1 * old + x1 * now;
     }
   }
   if (GROUPS > 1) {
@@ -493,10 +493,8 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
     for (int w = 0; w < GROUPS; ++w) {
       const float f = __builtin_amdgcn_exp2f(ml_lds[group + w][0] - top);
       sum += ml_lds[group + w][1] * f;
-      if (f != 0.f) {
-        y0 += *(const f32x4*)y_lds[group + w][lane] * f;
-        y1 += *(const f32x4*)(y_lds[group + w][lane] + 4) * f;
-      }
+      y0 += *(const f32x4*)y_lds[group + w][lane] * f;
+      y1 += *(const f32x4*)(y_lds[group + w][lane] + 4) * f;
     }
   }
   if (token >= a.S) return;
@@ -567,7 +565,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
   a.row_tiles = (S * a.G + p.rows - 1) / p.rows;
   const int64_t units = (int64_t)B * Hkv * a.row_tiles;
-  PBS_REQUIRE(units < (1 << 24), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
+  PBS_REQUIRE(units < (1 << 22), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
   // the line of steps that workers share has to fit 32 bits, whatever the lengths turn out to be: a call that may not is not cut
   if (units * ((int64_t)max_pages * page_size / step_of(p.rows, kv_bits) + 1) > INT32_MAX) p.workers = 0;
   a.workers = p.workers;

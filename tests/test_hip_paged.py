@@ -266,6 +266,50 @@ def test_pages_outside_the_pool_and_behind_the_table(dev, form):
         assert torch.equal(f.pages.k.view(torch.uint8), before[0].view(torch.uint8)) and torch.equal(f.pages.v.view(torch.uint8), before[1].view(torch.uint8))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("S", [1, 20])
+def test_sequences_that_share_their_first_pages(dev, form, S):
+    """Three sequences behind the same 128 tokens, written once: each appends to pages of its own."""
+    g = torch.Generator(device="cuda").manual_seed(S)
+    pages = _garbage(alloc_pages(9, 2, 64, form))
+    table = torch.tensor([[4, 7, 0], [4, 7, 2], [4, 7, 8]], dtype=torch.int32, device="cuda")
+    ops.paged_append(pages, table[:1], _ints(0), _randn(g, 1, 2, 128, 128), _randn(g, 1, 2, 128, 128))
+    k, v, q = _randn(g, 3, 2, S, 128), _randn(g, 3, 2, S, 128), _randn(g, 3, 8, S, 128)
+    ops.paged_append(pages, table, _ints(128, 128, 128), k, v)
+    out = ops.paged_attn(q, pages, table, _ints(128, 128, 128))
+    for b in range(3):
+        kk, vv = tokens_of(pages, table[b].tolist(), 128 + S)
+        want, tol = attention(q[b], kk, vv, 128, S, 128 ** -0.5)
+        assert ((out[b].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("S", [1, 20])
+@pytest.mark.parametrize("past", [40, 3000])
+def test_infinities_and_nans_reach_the_rows_that_see_them(dev, form, S, past):
+    f = Filled(form, 8, 2, S, [past, past])
+    clean = f.attn()
+    f.q[0, 3, 0, 17] = float("nan")                 # one query row
+    out = f.attn()
+    assert out[0, 3, 0].isnan().all()
+    out[0, 3, 0] = clean[0, 3, 0]
+    assert torch.equal(out, clean)
+    f.q[0, 3, 0, 17] = 0.5
+    k = torch.zeros(2, 2, 1, 128, dtype=torch.bfloat16, device="cuda")
+    k[1, 0, 0, 5] = float("inf")
+    last = f.past + S - 1                           # the last token's key, which only the last query sees: head 0 of the second sequence
+    v = ops.paged_read(f.pages, f.table, f.past + S, past + S)[1][:, :, -1:].contiguous()
+    before = f.attn()
+    ops.paged_append(f.pages, f.table, last, k, v)
+    out = f.attn()
+    assert torch.equal(out[:, :, :-1], before[:, :, :-1]) and out[0].isfinite().all() and out[1, 4:].isfinite().all()
+    if form == "fp4":                               # (the group is held as NaN)
+        assert out[1, :4, -1].isnan().all()
+    else:
+        want = torch.where(f.q[1, :4, -1, 5:6] > 0, float("nan"), 0.0).expand(4, 128)   # weight exp(inf - inf), or exp(-inf)
+        assert torch.equal(out[1, :4, -1].isnan(), want.isnan())
+
+
 def test_pools_past_4_gib(dev):
     """Byte offsets past 32 bits, element offsets past 31: the pages used are the last of a pool of 9000 pages of half a megabyte."""
     pages = alloc_pages(9000, 8, 256, "bf16")
@@ -305,16 +349,17 @@ def test_a_step_on_another_stream_and_two_at_once(dev, form):
 
 
 @pytest.mark.parametrize("form", FORMS)
-def test_a_captured_decoding_step(dev, form):
+@pytest.mark.parametrize("S", [1, 9, 40])     # a wave's rows (one row tile; three), and rows through LDS
+def test_a_captured_decoding_step(dev, form, S):
     """Append and attention in a graph: replayed while the lengths grow, with eager work on the same pages between the replays."""
     g = torch.Generator(device="cuda").manual_seed(9)
     B, Hq, Hkv, page, steps = 2, 8, 2, 32, 6
-    pages = _garbage(alloc_pages(40, Hkv, page, form))
-    table = _table(g, B, 10, 40)
+    pages = _garbage(alloc_pages(120, Hkv, page, form))
+    table = _table(g, B, 55, 120)          # (room for more tokens than a single workgroup takes)
     past = _ints(60, 200)
     ops.paged_append(pages, table, _ints(0, 0), _randn(g, B, Hkv, 200, 128), _randn(g, B, Hkv, 200, 128), new_lens=past)
-    q, k, v = _randn(g, B, Hq, 1, 128), _randn(g, B, Hkv, 1, 128), _randn(g, B, Hkv, 1, 128)
-    angle = torch.rand(B, 1, 128, generator=g, device="cuda")
+    q, k, v = _randn(g, B, Hq, S, 128), _randn(g, B, Hkv, S, 128), _randn(g, B, Hkv, S, 128)
+    angle = torch.rand(B, S, 128, generator=g, device="cuda")
     cos, sin = angle.cos().to(torch.bfloat16), angle.sin().to(torch.bfloat16)
 
     def step():
@@ -334,10 +379,10 @@ def test_a_captured_decoding_step(dev, form):
         eager = step()[1]
         assert torch.equal(eager, got)
         for b, n in enumerate(past.tolist()):
-            kk, vv = tokens_of(pages, table[b].tolist(), n + 1)
-            want, tol = attention(q_rot[b], kk, vv, n, 1, 128 ** -0.5)
+            kk, vv = tokens_of(pages, table[b].tolist(), n + S)
+            want, tol = attention(q_rot[b], kk, vv, n, S, 128 ** -0.5)
             assert ((got[b].double() - want).abs() <= tol).all(), (i, b)
-        past += 1
+        past += S
 
 
 @pytest.mark.parametrize("form", FORMS)

@@ -55,11 +55,13 @@ def test_arguments_that_the_library_refuses():
                          (dict(k_out=FAKE + 8), b"aligned"), (dict(Hq=65535, Hkv=65535), b"too many heads")]:
         assert _append(lib, **change) == -1 and word in lib.pbs_last_error(), (change, lib.pbs_last_error())
     for change, word in [(dict(q=None), b"null"), (dict(out=None), b"null"), (dict(past=None), b"null"), (dict(S=0), b"shape"), (dict(Hq=5), b"shape"),
-                         (dict(Hq=0), b"shape"), (dict(S=1 << 26, Hq=4, Hkv=1), b"too many query rows"), (dict(scale=0.0), b"softmax_scale"),
+                         (dict(Hq=0), b"shape"), (dict(S=1 << 26, Hq=4, Hkv=1), b"too many query rows"), (dict(B=65535, Hq=65, Hkv=65), b"too many query rows"),
+                         (dict(max_len=0), b"max_len"), (dict(max_len=5000, n=1000), b"workspace"), (dict(max_len=5000, ws=FAKE + 128), b"workspace"),
+                         (dict(scale=0.0), b"softmax_scale"),
                          (dict(scale=-1.0), b"softmax_scale"), (dict(scale=float("nan")), b"softmax_scale"), (dict(scale=float("inf")), b"softmax_scale"),
                          (dict(strides=[512, 128, 128, 512, 128, 129]), b"strides"), (dict(q=FAKE + 8), b"aligned")]:
         assert _attn(lib, **change) == -1 and word in lib.pbs_last_error(), (change, lib.pbs_last_error())
-    for change, word in [(dict(lens=None), b"null"), (dict(k=None), b"null"), (dict(v=None), b"null"), (dict(L=0), b"shape"), (dict(v=FAKE + 8), b"aligned")]:
+    for change, word in [(dict(lens=None), b"null"), (dict(k=None), b"null"), (dict(v=None), b"null"), (dict(L=0), b"shape"), (dict(L=(1 << 28) + 1), b"shape"), (dict(v=FAKE + 8), b"aligned")]:
         assert _read(lib, **change) == -1 and word in lib.pbs_last_error(), (change, lib.pbs_last_error())
 
 

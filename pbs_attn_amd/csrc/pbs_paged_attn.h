@@ -4,6 +4,9 @@
 #include "pbs_wave.h"
 #include <float.h>
 
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
 constexpr int PAGED_WAVES = 4;       // of a workgroup
 constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences, at most: two a compute unit
 // A row's exponent is taken up where a logit is more than this above it (log2): weights stay below 2^8, which costs their sums in fp32 and their
@@ -43,6 +46,147 @@ __device__ __forceinline__ int paged_lane() {
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
   return l;
 }
+
+// What a lane holds of a tile of 32 tokens.  n = lane % 16, g = lane / 16.
+template <int BITS>
+struct Tile;
+template <>
+struct Tile<16> {
+  u32x4 k[8], v[8];
+};
+template <>
+struct Tile<4> {
+  u32x4 k[2], v[2];
+  uint32_t ks;
+  u32x2 vs;
+};
+__device__ __forceinline__ void load_k(Tile<16>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* k = p.k + at * paged_tile_bytes<16>() + n * 512 + g * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t.k[h * 4 + c] = *(const u32x4*)(k + h * 256 + c * 64);
+}
+__device__ __forceinline__ void load_v(Tile<16>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* v = p.v + at * paged_tile_bytes<16>() + g * 2048 + n * 16;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) t.v[d] = *(const u32x4*)(v + d * 256);
+}
+__device__ __forceinline__ void load_k(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* k = p.k + at * paged_tile_bytes<4>() + n * 128 + g * 16;
+  t.k[0] = *(const u32x4*)k;
+  t.k[1] = *(const u32x4*)(k + 64);
+  t.ks = *(const uint16_t*)(p.ks + at * 128 + g * 32 + n * 2);
+}
+__device__ __forceinline__ void load_v(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* v = p.v + at * paged_tile_bytes<4>() + g * 512 + n * 16;
+  t.v[0] = *(const u32x4*)v;
+  t.v[1] = *(const u32x4*)(v + 256);
+  t.vs = *(const u32x2*)(p.vs + at * 128 + (n >> 2) * 32 + g * 8);
+}
+
+// 16 query rows as the matrix instruction's right operand
+template <int BITS>
+struct Rows;
+struct RowsLds {   // of the four waves, lane by lane
+  u32x4 q[4][64];
+  int scale[64];
+};
+template <>
+struct Rows<16> {
+  bf16x8 q[4];
+  __device__ __forceinline__ void put(RowsLds& lds, int lane) const {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) lds.q[c][lane] = __builtin_bit_cast(u32x4, q[c]);
+  }
+  __device__ __forceinline__ void get(const RowsLds& lds, int lane) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q[c] = __builtin_bit_cast(bf16x8, lds.q[c][lane]);
+  }
+  __device__ __forceinline__ void load(const uint16_t* row, int g) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u32x4 x = {};
+      if (row) x = *(const u32x4*)(row + c * 32 + g * 8);
+      q[c] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+};
+// For 4-bit keys the queries are the sum of two e4m3 numbers a channel: the matrix instruction then takes the keys as they lie in memory, with
+// their scales.  A bf16 value has 8 bits, e4m3 4: q = 2^e (hi + lo / 32) with hi = e4m3(q / 2^e) and lo the 4 bits that are left, exact down to 2^-21
+// of the row's largest channel (below it both halves are subnormal and lo is rounded).
+template <>
+struct Rows<4> {
+  i32x8 hi, lo;
+  int scale_hi;
+  __device__ __forceinline__ int scale_lo() const { return scale_hi == 255 ? 255 : scale_hi - 5; }
+  __device__ __forceinline__ void put(RowsLds& lds, int lane) const {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      lds.q[c][lane] = (u32x4){(uint32_t)hi[4 * c], (uint32_t)hi[4 * c + 1], (uint32_t)hi[4 * c + 2], (uint32_t)hi[4 * c + 3]};
+      lds.q[2 + c][lane] = (u32x4){(uint32_t)lo[4 * c], (uint32_t)lo[4 * c + 1], (uint32_t)lo[4 * c + 2], (uint32_t)lo[4 * c + 3]};
+    }
+    lds.scale[lane] = scale_hi;
+  }
+  __device__ __forceinline__ void get(const RowsLds& lds, int lane) {
+    const u32x4 a = lds.q[0][lane], b = lds.q[1][lane], c = lds.q[2][lane], d = lds.q[3][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi[e] = (int)a[e]; hi[4 + e] = (int)b[e];
+      lo[e] = (int)c[e]; lo[4 + e] = (int)d[e];
+    }
+    scale_hi = lds.scale[lane];
+  }
+  __device__ __forceinline__ void load(const uint16_t* row, int g) {
+    u32x4 x[4] = {};   // channels 16 g .. 16 g + 15 and 64 + 16 g ..: 32 bytes of an 8-bit operand
+    if (row) {
+      x[0] = *(const u32x4*)(row + g * 16);
+      x[1] = *(const u32x4*)(row + g * 16 + 8);
+      x[2] = *(const u32x4*)(row + 64 + g * 16);
+      x[3] = *(const u32x4*)(row + 64 + g * 16 + 8);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(x[i][e] & 0x7fffu, (x[i][e] >> 16) & 0x7fffu));
+    TwoOf t = with_lane_xor<16>(top);
+    top = max(t.a, t.b);
+    t = with_lane_xor<32>(top);
+    top = max(t.a, t.b);
+    const int field = max((int)(top >> 7), 20);
+    const float up = __uint_as_float((uint32_t)(261 - field) << 23);   // the row's largest magnitude becomes 128 .. 256
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t a = x[w >> 1][(w & 1) * 2], b = x[w >> 1][(w & 1) * 2 + 1];
+      const float y0 = bf16_bits_to_f32(a & 0xffffu) * up, y1 = __uint_as_float(a & 0xffff0000u) * up;
+      const float y2 = bf16_bits_to_f32(b & 0xffffu) * up, y3 = __uint_as_float(b & 0xffff0000u) * up;
+      int h = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+      h = __builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, h, true);
+      int l = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 32.f, (y1 - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 32.f, 0, false);
+      l = __builtin_amdgcn_cvt_pk_fp8_f32((y2 - __builtin_amdgcn_cvt_f32_fp8(h, 2)) * 32.f, (y3 - __builtin_amdgcn_cvt_f32_fp8(h, 3)) * 32.f, l, true);
+      hi[w] = h;
+      lo[w] = l;
+    }
+    scale_hi = field >= 255 ? 255 : field - 7;    // (an infinity or NaN among the queries: NaN)
+  }
+};
+
+// S^T of one half (16 keys, operand row m = token 2 m + half) and 16 query rows
+__device__ __forceinline__ f32x4 logits(const Tile<16>& t, int half, const Rows<16>& r) {
+  f32x4 s = {};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[half * 4 + c]), r.q[c], s, 0, 0, 0);
+  return s;
+}
+template <int HALF>
+__device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
+  const i32x8 k = {(int)t.k[HALF][0], (int)t.k[HALF][1], (int)t.k[HALF][2], (int)t.k[HALF][3], 0, 0, 0, 0};
+  f32x4 s = {};
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo());
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 4, 0, HALF, (int)t.ks, 0, r.scale_hi);
+}
+__device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
 
 // a sequence, and one of its row tiles
 struct PagedSeq {

@@ -1,8 +1,12 @@
 // Attention over a paged cache for prompts behind a filled cache and drafted tokens: 64 or 128 query rows a workgroup.
 //
 // The mathematics and the row numbering are those of pbs_paged_attn.hip.  Here the waves share the keys and split the rows (16 or 32 each), so
-// tiles of 64 keys go through LDS, two buffers of 32 KB: bf16 tiles are copied there asynchronously, 4-bit ones are loaded into registers
-// during the tile before and unpacked to bf16 behind it, once for all rows.
+// tiles of 64 keys go through LDS, two buffers: bf16 tiles are copied there asynchronously; values in 4 bits are loaded into registers during
+// the tile before and unpacked to bf16 behind it, once for all rows, while keys in 4 bits need no unpacking and go to every wave's registers
+// as they are.
+//
+// A wave's order within a step keeps both units busy: the logits of its second 32 keys beside the weights of the first, the products of the
+// first beside the weights of the second.
 #include "pbs_paged_attn.h"
 #include <math.h>
 
@@ -10,15 +14,13 @@ namespace {
 
 constexpr int WAVES = PAGED_WAVES;
 constexpr int KEYS = 64;                      // of a step
-constexpr int LDS_V = KEYS * PAGED_D * 2;     // V behind K in a buffer
-constexpr int LDS_BUFFER = 2 * LDS_V;
-constexpr int LDS_SHARE = 2 * LDS_BUFFER;
-constexpr int LDS_TOTAL = LDS_SHARE + (int)sizeof(PagedShareLds);
+constexpr int lds_v(int bits) { return bits == 16 ? KEYS * PAGED_D * 2 : 0; }   // V, behind K, in a buffer
+constexpr int lds_buffer(int bits) { return lds_v(bits) + KEYS * PAGED_D * 2; }
+constexpr int lds_total(int bits) { return 2 * lds_buffer(bits) + (int)sizeof(PagedShareLds); }
 
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 extern __shared__ __attribute__((aligned(16))) char lds[];
 
-// K rows of 256 bytes, the 16-byte chunk j of row r in place j ^ (r / 2 % 16): an operand's sixteen lanes read rows 2 n + half.
+// bf16 K: rows of 256 bytes, the 16-byte chunk j of row r in place j ^ (r / 2 % 16): an operand's sixteen lanes read rows 2 n + half.
 __device__ __forceinline__ int k_place(int row, int chunk) { return row * 256 + ((chunk ^ ((row >> 1) & 15)) * 16); }
 
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
@@ -54,40 +56,25 @@ struct Stage<16> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) copy_async(k, k_from[i], buffer + (uint32_t)(wave * 4096 + i * 1024));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) copy_async(v, (uint32_t)(lane * 16 + i * 1024), buffer + (uint32_t)(LDS_V + wave * 4096 + i * 1024));
+    for (int i = 0; i < 4; ++i) copy_async(v, (uint32_t)(lane * 16 + i * 1024), buffer + (uint32_t)(lds_v(16) + wave * 4096 + i * 1024));
   }
   __device__ __forceinline__ void store(uint32_t buffer, int held0, int held1) {}   // (the copies are awaited by all waves before the barrier)
 };
 template <>
 struct Stage<4> {
-  u32x4 k, v[2];
-  uint32_t ks;
+  u32x4 v[2];
   u32x2 vs;
   __device__ __forceinline__ void begin(int, int) {}
   __device__ __forceinline__ void load(const PagedPool& p, int64_t at0, int64_t at1, uint32_t, int, int) {
-    {   // K: a token's group of 32 channels
-      const int row = threadIdx.x >> 2, q4 = threadIdx.x & 3;
-      const int64_t at = row < 32 ? at0 : at1;
-      k = *(const u32x4*)(p.k + at * paged_tile_bytes<4>() + (row & 31) * 64 + q4 * 16);
-      ks = p.ks[at * 128 + q4 * 32 + (row & 31)];
-    }
-    {   // V: eight tokens of channels 8 m .. 8 m + 7, of which a thread unpacks four
-      const int m = threadIdx.x & 15, eight = (threadIdx.x >> 4) & 7;
-      const int64_t at = eight < 4 ? at0 : at1;
-      const char* src = p.v + at * paged_tile_bytes<4>() + (eight & 3) * 512 + m * 16;
-      v[0] = *(const u32x4*)src;
-      v[1] = *(const u32x4*)(src + 256);
-      vs = *(const u32x2*)(p.vs + at * 128 + (m >> 2) * 32 + (eight & 3) * 8);
-    }
+    const int m = threadIdx.x & 15, eight = (threadIdx.x >> 4) & 7;   // eight tokens of channels 8 m .. 8 m + 7, of which a thread unpacks four
+    const int64_t at = eight < 4 ? at0 : at1;
+    const char* src = p.v + at * paged_tile_bytes<4>() + (eight & 3) * 512 + m * 16;
+    v[0] = *(const u32x4*)src;
+    v[1] = *(const u32x4*)(src + 256);
+    vs = *(const u32x2*)(p.vs + at * 128 + (m >> 2) * 32 + (eight & 3) * 8);
   }
   // `held`: tokens of either half that are there; scales of the others are 2^-127, as they may be NaN and codes are not
   __device__ __forceinline__ void store(uint32_t buffer, int held0, int held1) {
-    {
-      const int row = threadIdx.x >> 2, q4 = threadIdx.x & 3;
-      const float e = __uint_as_float(ks << 23);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) *(u32x4*)(lds + buffer + k_place(row, q4 * 4 + w)) = fp4_values(k[w], e);
-    }
     const int m = threadIdx.x & 15, eight = (threadIdx.x >> 4) & 7, half = threadIdx.x >> 7;
     const int held = (eight < 4 ? held0 : held1) - (eight & 3) * 8;
     bf16x2 x[8][2];
@@ -108,7 +95,7 @@ struct Stage<4> {
         lo[w] = __builtin_amdgcn_perm(b, a, 0x05040100u);
         hi[w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
       }
-      char* dst = lds + buffer + LDS_V + (eight * PAGED_D + (4 * half + 2 * c) * 16 + m) * 16;
+      char* dst = lds + buffer + lds_v(4) + (eight * PAGED_D + (4 * half + 2 * c) * 16 + m) * 16;
       *(u32x4*)dst = lo;
       *(u32x4*)(dst + 256) = hi;
     }
@@ -120,7 +107,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   constexpr int ROWS = WAVES * RW * 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const float c = a.scale_log2;
-  bf16x8 q[RW][4];
+  Rows<BITS> q[RW];
   f32x4 o[RW][8];
   float m[RW];
   f32x4 l[RW];   // the weights' sums, as products with ones (every row of the tile the same): 32 bits, on the matrix unit, and no sum over lanes
@@ -129,13 +116,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   for (int r = 0; r < RW; ++r) {
     const int row = u.r0 + (wave * RW + r) * 16 + n, token = row / a.G;
     const bool valid = token < u.fresh;
-    const uint16_t* src = a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss + g * 8;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      u32x4 x = {};
-      if (valid) x = *(const u32x4*)(src + k * 32);
-      q[r][k] = __builtin_bit_cast(bf16x8, x);
-    }
+    q[r].load(valid ? a.q + u.b * a.q_sb + (head * a.G + row % a.G) * a.q_sh + (int64_t)token * a.q_ss : nullptr, g);
     seen[r] = valid ? u.past + token + 1 : 0;
     m[r] = -FLT_MAX;
     l[r] = (f32x4){};
@@ -161,26 +142,31 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   int64_t at0, at1;
   int held0 = 0, held1 = 0, next0 = 0, next1 = 0;
   uint32_t buffer = 0;
+  Tile<4> keys[2];   // (4 bits)
   if (s0 < end) {
     look_up(s0, at0, at1, held0, held1);
     stage.load(a.pool, at0, at1, buffer, wave, lane);
+    if (BITS == 4) {
+      load_k(keys[0], a.pool, at0, n, g);
+      load_k(keys[1], a.pool, at1, n, g);
+    }
     stage.store(buffer, held0, held1);
   }
   for (int step = s0; step < end; ++step) {
     // this tile's copies have landed, and nobody reads the other buffer any more.  (By the builtin: the compiler sees that the queries have
     // landed too, and does not wait for them behind the next copies, which it does not count.)
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    if (BITS == 16) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
     asm volatile("" ::: "memory");
     __syncthreads();
     if (step + 1 < end) {
       look_up(step + 1, at0, at1, next0, next1);
-      stage.load(a.pool, at0, at1, buffer ^ LDS_BUFFER, wave, lane);
+      stage.load(a.pool, at0, at1, buffer ^ lds_buffer(BITS), wave, lane);
     }
     if (BITS == 16 && held0 + held1 < KEYS) {
       // tokens that are not there hold whatever the page held before: not even times zero
       for (int i = threadIdx.x; i < KEYS / 8 * PAGED_D; i += 256) {
         const int held = (i < 4 * PAGED_D ? held0 : held1) - (i / PAGED_D & 3) * 8;
-        u32x4* x = (u32x4*)(lds + buffer + LDS_V) + i;
+        u32x4* x = (u32x4*)(lds + buffer + lds_v(BITS)) + i;
         if (held < 8) {
 #pragma unroll
           for (int w = 0; w < 4; ++w) (*x)[w] &= held >= 2 * w + 2 ? 0xffffffffu : held == 2 * w + 1 ? 0xffffu : 0u;
@@ -189,79 +175,101 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       __syncthreads();
     }
     const int k0 = step * KEYS;
-    const bool whole = k0 + KEYS <= u.all_see && held0 + held1 == KEYS;
     const char* kt = lds + buffer;
-    const char* vt = lds + buffer + LDS_V;
+    const char* vt = lds + buffer + lds_v(BITS);
     // Operands are read from LDS two groups of four ahead of the products that take them; the fences keep the compiler from sinking the reads.
     f32x4 s[RW][2][2];
-    bf16x8 k[3][4], v[3][4];
+    bf16x8 k[3][4], v[3][4], p[RW][2];
+    auto fence = [] __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
     auto read_k = [&](int i) __attribute__((always_inline)) {
       // operand row n is token 32 (i / 2) + 2 n + i % 2: a lane ends up with the logits of eight tokens in a row, 32 (i / 2) + 8 g ..
+      if (BITS == 16) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) k[i % 3][e] = *(const bf16x8*)(kt + k_place(32 * (i >> 1) + 2 * n + (i & 1), e * 4 + g));
+        for (int e = 0; e < 4; ++e) k[i % 3][e] = *(const bf16x8*)(kt + k_place(32 * (i >> 1) + 2 * n + (i & 1), e * 4 + g));
+      }
     };
     auto read_v = [&](int i) __attribute__((always_inline)) {   // channels 16 d + n, d = 4 (i % 2) .., of tokens 32 (i / 2) + 8 g ..
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[i % 3][e] = *(const bf16x8*)(vt + ((4 * (i >> 1) + g) * PAGED_D + (4 * (i & 1) + e) * 16 + n) * 16);
     };
-    auto fence = [] __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
-    read_k(0);
-    read_k(1);
+    auto multiply = [&](int i) __attribute__((always_inline)) {
+      if constexpr (BITS == 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fence();
-      if (i < 2) read_k(i + 2);
-      else read_v(i - 2);
+        for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = (f32x4){};
 #pragma unroll
-      for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = (f32x4){};
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+          for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % 3][e], q[r].q[e], s[r][i >> 1][i & 1], 0, 0, 0);
+      } else {
 #pragma unroll
-        for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % 3][e], q[r][e], s[r][i >> 1][i & 1], 0, 0, 0);
-    }
-    fence();
-    if (!whole) {
-#pragma unroll
-      for (int r = 0; r < RW; ++r)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = 8 * g + j;
-            const bool there = key < (i ? held1 : held0) && k0 + 32 * i + key < seen[r];
-            if (!there) s[r][i][j & 1][j >> 1] = -INFINITY;
-          }
-    }
-    bf16x8 p[RW][2];
-    float top[RW];
-    bool grows = false;
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      top[r] = s[r][0][0][0];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], s[r][i][j & 1][j >> 1]);
-      grows |= top[r] * c > m[r] + PAGED_SLACK;   // (this lane's keys; the row's are looked at where one of them is)
-    }
-    if (__any(grows)) {
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        const float m_new = fmaxf(m[r], max_over_groups(top[r]) * c), f = __builtin_amdgcn_exp2f(m[r] - m_new);
-        l[r] *= f;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) o[r][d] *= f;
-        m[r] = m_new;
+        for (int r = 0; r < RW; ++r) s[r][i >> 1][i & 1] = logits(keys[i >> 1], i & 1, q[r]);
       }
-    }
+    };
     auto weigh = [&](int r, int i) __attribute__((always_inline)) {
       // half a step of 2^-8 off, above the line and below it
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
     };
-    // weights of the first 32 keys; then their products, and beside them the weights of the other 32
+    // 32 keys' masks and maxima.  Where the second 32's grow, the weights of the first, which have not been multiplied yet, are taken again.
+    auto look = [&](int i) __attribute__((always_inline)) {
+      const int held = i ? held1 : held0, first = k0 + 32 * i;
+      if (first + PAGED_TILE > u.all_see || held < PAGED_TILE) {
 #pragma unroll
-    for (int r = 0; r < RW; ++r) weigh(r, 0);
+        for (int r = 0; r < RW; ++r) {
+          const int there = min(held, seen[r] - first) - 8 * g;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j >= there) s[r][i][j & 1][j >> 1] = -INFINITY;
+        }
+      }
+      float top[RW];
+      bool grows = false;
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        top[r] = s[r][i][0][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top[r] = fmaxf(top[r], s[r][i][j & 1][j >> 1]);
+        grows |= top[r] * c > m[r] + PAGED_SLACK;   // (this lane's keys; the row's are looked at where one of them is)
+      }
+      if (__any(grows)) {
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const float most = max_over_groups(top[r]) * c;
+          const float m_new = most > m[r] + PAGED_SLACK ? most : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
+          l[r] *= f;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) o[r][d] *= f;
+          m[r] = m_new;
+          if (i == 1) weigh(r, 0);
+        }
+      }
+    };
+    read_k(0);
+    read_k(1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fence();
+      read_k(i + 2);
+      multiply(i);
+    }
+    fence();
+    look(0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fence();
+      read_v(i);
+      multiply(i + 2);
+      if (i < RW) {
+        weigh(i, 0);
+        asm volatile("" : "+v"(p[i][0]));   // (here, and not behind the branch that may take them again)
+      }
+    }
+    fence();
+    if (BITS == 4 && step + 1 < end) {
+      load_k(keys[0], a.pool, at0, n, g);
+      load_k(keys[1], a.pool, at1, n, g);
+    }
+    look(1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       fence();
@@ -280,7 +288,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     fence();
     held0 = next0;
     held1 = next1;
-    buffer ^= LDS_BUFFER;
+    buffer ^= lds_buffer(BITS);
     if (step + 1 < end) stage.store(buffer, held0, held1);
   }
 
@@ -318,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(PagedAttnArgs a) {
   // Workers that follow each other read the same head's keys at the same time: they go to one of the eight dies and its L2 (workgroups
   // are dealt to them in turn).  Without cuts the heads follow each other, and the row tiles that see the most keys come first.
   const int worker = a.headers ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : 0;
-  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true,
+  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + 2 * lds_buffer(BITS)), worker, true,
                                   [&](const PagedUnit& u, int head, int step, int steps, float* part)
                                   __attribute__((always_inline)) { work<BITS, RW>(a, u, head, step, steps, part); });
 }
@@ -327,11 +335,11 @@ template <int BITS, int RW>
 int launch(const PagedAttnArgs& a, hipStream_t stream) {
   const void* kernel = (const void*)attn_rows_kernel<BITS, RW>;
   if (const int rc = pbs_require_no_static_lds(kernel, "pbs_paged_attn_fwd")) return rc;
-  if (const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_TOTAL); e != hipSuccess) {
+  if (const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds_total(BITS)); e != hipSuccess) {
     pbs_set_error("pbs_paged_attn_fwd: hipFuncSetAttribute: %s", hipGetErrorString(e));
     return (int)e;
   }
-  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), dim3(a.headers ? a.workers : a.Hkv * a.B * a.row_tiles), dim3(256), LDS_TOTAL, stream, a);
+  hipLaunchKernelGGL((attn_rows_kernel<BITS, RW>), dim3(a.headers ? a.workers : a.Hkv * a.B * a.row_tiles), dim3(256), lds_total(BITS), stream, a);
   return 0;
 }
 

@@ -362,7 +362,8 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
 }
 
 // Steps of a row tile of `rows`
-constexpr int step_of(int rows, int kv_bits) { return rows > 48 ? 64 : rows == 16 && kv_bits == 4 ? 256 : 128; }
+constexpr bool through_lds(int rows, int kv_bits) { return rows > (kv_bits == 16 ? 32 : 64); }
+constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : rows == 16 && kv_bits == 4 ? 256 : 128; }
 
 struct Plan {
   int rows;      // of a row tile
@@ -372,11 +373,11 @@ struct Plan {
 Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : rows <= 64 ? 64 : 128;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits == 4 ? 48 : rows <= 64 ? 64 : 128;
   // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512
   // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  const bool cut = max_len > (kv_bits == 16 ? 640 : 1280) && (p.rows <= 48 || units < 4 * PAGED_WORKERS);
+  const bool cut = max_len > (kv_bits == 16 ? 640 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // (no more workers than there is work for)
   const int64_t steps = units * ((max_len + step_of(p.rows, kv_bits) - 1) / step_of(p.rows, kv_bits));
   p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS, steps + 7) / 8 * 8 : 0;
@@ -429,21 +430,23 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.headers = p.workers ? (PagedHeader*)workspace : nullptr;
   a.parts = p.workers ? (float*)((char*)workspace + p.workers * sizeof(PagedHeader)) : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  if (p.rows > 48) {
+  if (through_lds(p.rows, kv_bits)) {
     if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
   } else if (kv_bits == 16) {
     if (p.rows == 16) launch<16, 1, 1>(a, st);
-    else if (p.rows == 32) launch<16, 2, 1>(a, st);
-    else launch<16, 3, 1>(a, st);
+    else launch<16, 2, 1>(a, st);
   } else {
     if (p.rows == 16) launch<4, 1, 2>(a, st);
     else if (p.rows == 32) launch<4, 2, 1>(a, st);
-    else launch<4, 3, 1>(a, st);
+    else if (p.rows == 48) launch<4, 3, 1>(a, st);
+    else launch<4, 4, 1>(a, st);
   }
   if (p.workers) {
     const int rows = (int)std::min<int64_t>(p.rows, (int64_t)S * a.G);
-    if (p.rows == 16) hipLaunchKernelGGL(join_kernel<16>, dim3(p.workers, rows), dim3(256), 0, st, a, p.rows);
-    else if (p.rows <= 48) hipLaunchKernelGGL(join_kernel<4>, dim3(p.workers, (rows + 3) / 4), dim3(256), 0, st, a, p.rows);
+    // (parts of a row, if sequences are alike: with 32 heads' rows of one sequence, 4 KV heads, 128)
+    const int64_t parts = p.workers / units;
+    if (parts >= 32) hipLaunchKernelGGL(join_kernel<16>, dim3(p.workers, rows), dim3(256), 0, st, a, p.rows);
+    else if (parts >= 4) hipLaunchKernelGGL(join_kernel<4>, dim3(p.workers, (rows + 3) / 4), dim3(256), 0, st, a, p.rows);
     else hipLaunchKernelGGL(join_kernel<1>, dim3(p.workers, (rows + 15) / 16), dim3(256), 0, st, a, p.rows);
   }
   return pbs_check_launch("pbs_paged_attn_fwd");

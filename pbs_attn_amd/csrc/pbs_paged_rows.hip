@@ -347,5 +347,5 @@ int launch(const PagedAttnArgs& a, hipStream_t stream) {
 
 int paged_attn_rows(const PagedAttnArgs& a, int kv_bits, int rows, hipStream_t stream) {
   if (kv_bits == 16) return rows == 64 ? launch<16, 1>(a, stream) : launch<16, 2>(a, stream);
-  return rows == 64 ? launch<4, 1>(a, stream) : launch<4, 2>(a, stream);
+  return launch<4, 2>(a, stream);
 }

@@ -208,6 +208,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
     }
+    __builtin_amdgcn_sched_barrier(0);   // (or the loads sink behind the products: 35 rows 61.2 -> 59.7 us)
     s.template add<mask.value>(tile, p, k0, u.keys, gone, g);
     if (load) {
 #pragma unroll
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
 
 // Steps of a row tile of `rows`
 constexpr bool through_lds(int rows, int kv_bits) { return rows > (kv_bits == 16 ? 32 : 64); }
-constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : rows == 16 && kv_bits == 4 ? 256 : 128; }
+constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : kv_bits == 4 && rows <= 48 ? 256 : 128; }
 
 struct Plan {
   int rows;      // of a row tile
@@ -385,10 +386,11 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   return p;
 }
 
-template <int BITS, int R, int NT>
+// NT tiles a wave and step, DEPTH steps ahead, where sequences are cut; without cuts there are eight waves and one step fewer registers
+template <int BITS, int R, int NT, int DEPTH>
 void launch(const PagedAttnArgs& a, hipStream_t stream) {
-  if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, NT, 4>), dim3(a.workers), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((attn_kernel<BITS, R, NT, NT, 8>), dim3(a.Hkv * a.B * a.row_tiles), dim3(512), 0, stream, a);
+  if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), dim3(a.workers), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), dim3(a.Hkv * a.B * a.row_tiles), dim3(512), 0, stream, a);
 }
 
 }  // namespace
@@ -433,13 +435,13 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   if (through_lds(p.rows, kv_bits)) {
     if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
   } else if (kv_bits == 16) {
-    if (p.rows == 16) launch<16, 1, 1>(a, st);
-    else launch<16, 2, 1>(a, st);
+    if (p.rows == 16) launch<16, 1, 1, 1>(a, st);
+    else launch<16, 2, 1, 1>(a, st);
   } else {
-    if (p.rows == 16) launch<4, 1, 2>(a, st);
-    else if (p.rows == 32) launch<4, 2, 1>(a, st);
-    else if (p.rows == 48) launch<4, 3, 1>(a, st);
-    else launch<4, 4, 1>(a, st);
+    if (p.rows == 16) launch<4, 1, 2, 2>(a, st);
+    else if (p.rows == 32) launch<4, 2, 2, 1>(a, st);
+    else if (p.rows == 48) launch<4, 3, 2, 1>(a, st);
+    else launch<4, 4, 1, 1>(a, st);
   }
   if (p.workers) {
     const int rows = (int)std::min<int64_t>(p.rows, (int64_t)S * a.G);

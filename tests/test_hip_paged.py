@@ -188,6 +188,9 @@ def test_read_gives_the_tokens_and_zeros_behind_them(dev, form, page):
     (5, 1, 3, [61], None, 32),                           # 15 rows
     (28, 4, 5, [100, 40], [5, 2], 64),                   # 35 rows: drafted tokens
     (20, 4, 2, [5000], None, 256),
+    (28, 4, 3, [90, 300], [3, 1], 128),                  # 21 rows
+    (28, 4, 7, [2, 400], [4, 7], 32),                    # 49 rows
+    (8, 1, 8, [600], None, 64),                          # 64 rows
     (8, 2, 33, [0, 200], [33, 30], 64),                  # prompts: rows that see few keys beside rows that see many
     (6, 2, 100, [1500, 0], [64, 100], 128),
     (4, 4, 257, [300], None, 64),
@@ -204,7 +207,9 @@ def test_attention_over_the_pages(dev, form, Hq, Hkv, S, past, new, page):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("B,Hq,Hkv,S,past", [(1, 8, 2, 1, 40000), (2, 4, 1, 3, 33333), (40, 28, 4, 1, 900), (1, 32, 8, 200, 5000)])
+@pytest.mark.parametrize("B,Hq,Hkv,S,past", [(1, 8, 2, 1, 40000), (2, 4, 1, 3, 33333), (40, 28, 4, 1, 900), (1, 32, 8, 200, 5000),
+                                             # every number of row tiles, a few long sequences beside short ones
+                                             (3, 28, 4, 3, 6000), (3, 28, 4, 5, 6000), (3, 28, 4, 9, 6000), (1, 28, 4, 9, 20000), (5, 28, 4, 20, 3000)])
 def test_attention_over_long_caches_and_many_sequences(dev, form, B, Hq, Hkv, S, past):
     g = torch.Generator().manual_seed(B)
     pasts = [past] + [int(torch.randint(0, past, (1,), generator=g)) for _ in range(B - 1)]

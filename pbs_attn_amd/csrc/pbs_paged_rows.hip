@@ -9,7 +9,7 @@
 // first beside the weights of the second.
 //
 // Bound by the matrix unit, and what keeps it from its rate is the softmax on the vector unit: 500 new tokens of two sequences behind up to 16k
-// (32 / 8 heads) 245 us, 860 TFLOP/s; 1000 behind 32k in 4 bits 596 us, 915 (without the order above 671, with the waits for the next
+// (32 / 8 heads) 239 us, 880 TFLOP/s; 1000 behind 32k in 4 bits 580 us, 940 (without the order above 671, with the waits for the next
 // tile's copies in front of each step's first product 700).  Of the time the matrix unit is busy half.
 #include "pbs_paged_attn.h"
 #include <math.h>
@@ -274,6 +274,8 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       load_k(keys[1], a.pool, at1, n, g);
     }
     look(1);
+    // (the wave that multiplies goes before the one that weighs: 246 -> 239 us, in 4 bits 595 -> 580; ahead of the logits' products too 242 and 588)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       fence();
@@ -289,6 +291,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         for (int r = 0; r < RW; ++r) l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i >> 1], l[r], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     fence();
     held0 = next0;
     held1 = next1;

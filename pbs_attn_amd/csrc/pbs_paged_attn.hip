@@ -284,6 +284,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       for (int w = 0; w < WAVES; ++w) y[e] += o_lds[w][rr][c + e];
     }
     if (part) {
+      if (token >= u.fresh) continue;   // (cleared by the join)
       float* dst = part + (r * 16 + rr) * PAGED_D + c;
       *(f32x4*)dst = (f32x4){y[0], y[1], y[2], y[3]};
       *(f32x4*)(dst + 4) = (f32x4){y[4], y[5], y[6], y[7]};
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
   const float* first = a.parts + ((int64_t)blockIdx.x * 2 + 1) * slot;
   float top = -FLT_MAX, sum = 0.f;
   f32x4 y0 = {}, y1 = {};
-  if (token < a.S) {
+  if (token < fresh) {
 #pragma unroll 4
     for (int i = share; i <= h.more; i += GROUPS) {
       // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on

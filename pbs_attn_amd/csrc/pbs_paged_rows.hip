@@ -304,6 +304,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     const float sum = l[r][0];
     const int rr = (wave * RW + r) * 16 + n, row = u.r0 + rr, token = row / a.G;
     if (part) {
+      if (token >= u.fresh) continue;   // (cleared by the join)
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll

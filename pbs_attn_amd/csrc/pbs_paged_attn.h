@@ -3,6 +3,8 @@
 #include "pbs_paged.h"
 #include "pbs_wave.h"
 #include <float.h>
+#include <limits.h>
+#include <math.h>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
@@ -84,6 +86,29 @@ __device__ __forceinline__ void load_v(Tile<4>& t, const PagedPool& p, int64_t a
   t.v[1] = *(const u32x4*)(v + 256);
   t.vs = *(const u32x2*)(p.vs + at * 128 + (n >> 2) * 32 + g * 8);
 }
+
+// Values that are not finite, of tokens that some of a row tile's rows do not see (the call's own): not even times zero.  They leave the tile that
+// is multiplied, and the rows that see one get it at the end: what a row sees begins with the first token, so the first key is enough.
+struct PagedLater {
+  int up[PAGED_D], down[PAGED_D];   // by channel: the first key that is an infinity or NaN, for `up` all but -inf, for `down` all but +inf
+  int any;
+
+  __device__ __forceinline__ void begin() {
+    if (threadIdx.x < PAGED_D) up[threadIdx.x] = down[threadIdx.x] = INT_MAX;
+    if (threadIdx.x == 0) any = 0;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void note(int channel, int key, uint32_t bits) {   // (bits of the bf16 value)
+    if (bits != 0xff80u) atomicMin(&up[channel], key);
+    if (bits != 0x7f80u) atomicMin(&down[channel], key);
+    any = 1;
+  }
+  __device__ __forceinline__ bool is_any() const { return __builtin_amdgcn_readfirstlane(any) != 0; }
+  __device__ __forceinline__ float of(int channel, int seen) const {
+    return (up[channel] < seen ? INFINITY : 0.f) - (down[channel] < seen ? INFINITY : 0.f);
+  }
+};
+__device__ __forceinline__ bool not_finite(uint32_t bf16_bits) { return (bf16_bits & 0x7f80u) == 0x7f80u; }
 
 // 16 query rows as the matrix instruction's right operand
 template <int BITS>

@@ -56,6 +56,32 @@ __device__ __forceinline__ void values(const Tile<4>& t, int c, int held, bf16x8
   v[0] = __builtin_bit_cast(bf16x8, lo);
   v[1] = __builtin_bit_cast(bf16x8, hi);
 }
+// infinities and NaN among the values of a lane's first `held` tokens, of which the first is `key`: noted, and out of the tile
+__device__ __forceinline__ void set_aside(Tile<16>& t, PagedLater& later, int key, int held, int n) {
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    u32x4 x = t.v[d];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = x[j >> 1] >> (16 * (j & 1)) & 0xffffu;
+      if (!not_finite(h)) continue;
+      if (j < held) later.note(d * 16 + n, key + j, h);
+      x[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+    }
+    t.v[d] = x;
+  }
+}
+__device__ __forceinline__ void set_aside(Tile<4>& t, PagedLater& later, int key, int held, int n) {   // (a token's group is NaN or finite)
+  u32x2 x = t.vs;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if ((x[j >> 2] >> (8 * (j & 3)) & 0xffu) != 0xffu) continue;
+    if (j < held)
+      for (int d = 0; d < 8; ++d) later.note(n * 8 + d, key + j, 0x7fffu);
+    x[j >> 2] &= ~(0xffu << (8 * (j & 3)));
+  }
+  t.vs = x;
+}
 template <int BITS>
 __device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? d * 16 + row : row * 8 + d; }
 
@@ -167,8 +193,10 @@ struct Softmax {
 // Steps `s0` .. `s0 + steps - 1` of a unit and head, WAVES * NT tiles a step, NT a wave; then the waves' sums together in LDS, and out, or as a part.
 template <int BITS, int R, int NT, int DEPTH, int WAVES>
 __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part,
-                                     float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2], RowsLds* q_lds) {
+                                     float (&o_lds)[WAVES][16][O_PITCH], float (&ml_lds)[WAVES][16][2], RowsLds* q_lds, PagedLater& later) {
   const int lane = paged_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const bool mixed = u.all_see < u.keys;   // (never with a single token)
+  if (mixed) later.begin();
   Softmax<BITS, R, NT> s;
   s.begin(a, u, head, n, g, wave, q_lds);
   const int tiles = (u.keys + PAGED_TILE - 1) / PAGED_TILE;
@@ -214,6 +242,13 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
     }
+    if (mask.value && mixed && k0 + NT * PAGED_TILE > u.all_see) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int key = k0 + i * PAGED_TILE + 8 * g;
+        set_aside(tile[i], later, key, gone >> i & 1 ? 0 : u.keys - key, n);
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);   // (or the loads sink behind the products: 35 rows 61.2 -> 59.7 us)
     s.template add<mask.value>(tile, p, k0, u.keys, gone, g);
     if (load) {
@@ -251,6 +286,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   loop(std::true_type{});
 
   const int lane2 = paged_lane(), n2 = lane2 & 15, g2 = lane2 >> 4;
+  bool noted = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float l = s.l[r][0];
@@ -269,6 +305,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
       for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = s.o[r][d][i] * f;
     __syncthreads();
+    if (r == 0) noted = mixed && later.is_any();
     // 16 lanes a row, 8 channels a lane
     const int rr = wave * 4 + g2, c = n2 * 8, row = u.r0 + r * 16 + rr, token = row / a.G;
     if (WAVES > 4 && wave >= 4) continue;
@@ -282,6 +319,10 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       y[e] = 0.f;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) y[e] += o_lds[w][rr][c + e];
+    }
+    if (noted) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] += later.of(c + e, u.past + token + 1);
     }
     if (part) {
       if (token >= u.fresh) continue;   // (cleared by the join)
@@ -308,8 +349,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_kernel(PagedAttnArgs a) {
   __shared__ float ml_lds[WAVES][16][2];
   __shared__ PagedShareLds share_lds;
   __shared__ RowsLds q_lds[R > 1 ? R : 1];
+  __shared__ PagedLater later;
   paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, false, [&](const PagedUnit& u, int head, int step, int steps, float* part)
-                                            __attribute__((always_inline)) { work<BITS, R, NT, DEPTH, WAVES>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds); });
+                                            __attribute__((always_inline)) { work<BITS, R, NT, DEPTH, WAVES>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds, later); });
 }
 
 // Joins the parts of every row tile and head that was cut: its first worker's beginning and the `more` workers' after it.  Sixteen lanes hold a
@@ -393,7 +435,7 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   return p;
 }
 
-// NT tiles a wave and step, DEPTH steps ahead, where sequences are cut; without cuts there are eight waves and one step fewer registers
+// NT tiles a wave and step, DEPTH steps ahead.  Without cuts a workgroup has eight waves, and several row tiles leave each half the registers.
 template <int BITS, int R, int NT, int DEPTH>
 void launch(const PagedAttnArgs& a, hipStream_t stream) {
   if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), dim3(a.workers), dim3(256), 0, stream, a);

@@ -20,7 +20,9 @@ constexpr int WAVES = PAGED_WAVES;
 constexpr int KEYS = 64;                      // of a step
 constexpr int lds_v(int bits) { return bits == 16 ? KEYS * PAGED_D * 2 : 0; }   // V, behind K, in a buffer
 constexpr int lds_buffer(int bits) { return lds_v(bits) + KEYS * PAGED_D * 2; }
-constexpr int lds_total(int bits) { return 2 * lds_buffer(bits) + (int)sizeof(PagedShareLds); }
+constexpr int lds_later(int bits) { return 2 * lds_buffer(bits); }
+constexpr int lds_share(int bits) { return lds_later(bits) + (int)sizeof(PagedLater); }
+constexpr int lds_total(int bits) { return lds_share(bits) + (int)sizeof(PagedShareLds); }
 
 extern __shared__ __attribute__((aligned(16))) char lds[];
 
@@ -111,6 +113,9 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   constexpr int ROWS = WAVES * RW * 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const float c = a.scale_log2;
+  PagedLater& later = *(PagedLater*)(lds + lds_later(BITS));
+  const bool mixed = u.all_see < u.keys;   // (not with rows of one token)
+  if (mixed) later.begin();
   Rows<BITS> q[RW];
   f32x4 o[RW][8];
   float m[RW];
@@ -179,6 +184,23 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       __syncthreads();
     }
     const int k0 = step * KEYS;
+    if (mixed && k0 + KEYS > u.all_see) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < KEYS / 8 * PAGED_D; i += 256) {
+        u32x4* at = (u32x4*)(lds + buffer + lds_v(BITS)) + i;
+        const int place = i % PAGED_D, key = k0 + i / PAGED_D * 8;
+        u32x4 x = *at;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t h = x[j >> 1] >> (16 * (j & 1)) & 0xffffu;
+          if (!not_finite(h)) continue;
+          later.note(BITS == 16 ? place : (place & 15) * 8 + (place >> 4), key + j, h);
+          x[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+        }
+        *at = x;
+      }
+      __syncthreads();
+    }
     const char* kt = lds + buffer;
     const char* vt = lds + buffer + lds_v(BITS);
     // Operands are read from LDS two groups of four ahead of the products that take them; the fences keep the compiler from sinking the reads.
@@ -299,10 +321,17 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     if (step + 1 < end) stage.store(buffer, held0, held1);
   }
 
+  const bool noted = mixed && later.is_any();   // (a step's barrier is behind its notes)
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
     const float sum = l[r][0];
     const int rr = (wave * RW + r) * 16 + n, row = u.r0 + rr, token = row / a.G;
+    if (noted) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[r][d][i] += later.of(BITS == 16 ? d * 16 + 4 * g + i : (4 * g + i) * 8 + d, u.past + token + 1);
+    }
     if (part) {
       if (token >= u.fresh) continue;   // (cleared by the join)
 #pragma unroll
@@ -334,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(PagedAttnArgs a) {
   // Workers that follow each other read the same head's keys at the same time: they go to one of the eight dies and its L2 (workgroups
   // are dealt to them in turn).  Without cuts the heads follow each other, and the row tiles that see the most keys come first.
   const int worker = a.headers ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : 0;
-  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + 2 * lds_buffer(BITS)), worker, true,
+  paged_go<WAVES * RW * 16, KEYS>(a, *(PagedShareLds*)(lds + lds_share(BITS)), worker, true,
                                   [&](const PagedUnit& u, int head, int step, int steps, float* part)
                                   __attribute__((always_inline)) { work<BITS, RW>(a, u, head, step, steps, part); });
 }

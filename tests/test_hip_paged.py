@@ -315,6 +315,34 @@ def test_infinities_and_nans_reach_the_rows_that_see_them(dev, form, S, past):
         assert torch.equal(out[1, :4, -1].isnan(), want.isnan())
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("S,past", [(2, 0), (4, 40), (7, 3000), (11, 40), (11, 3000), (16, 40), (16, 3000), (40, 0), (40, 3000), (75, 1030)])   # 8 .. 300 rows
+def test_values_that_are_not_finite_reach_no_earlier_row(dev, form, S, past):
+    """Infinities and NaN among the new tokens' values: rows before them keep their bits, rows from them on get them."""
+    f = Filled(form, 8, 2, S, [past, past])
+    clean = f.attn()
+    k, v = (x[:, :, past:].contiguous() for x in ops.paged_read(f.pages, f.table, f.past + S, past + S))
+    t = S // 2
+    v[1, 0, t, 5], v[1, 0, t, 38], v[1, 0, t, 71] = float("inf"), -float("inf"), float("nan")
+    v[1, 0, S - 1, 38] = float("inf")
+    ops.paged_append(f.pages, f.table, f.past, k, v)
+    out = f.attn()
+    if form == "bf16":
+        seen, last = out[1, :4, t:S - 1] if t < S - 1 else None, out[1, :4, S - 1]
+        if seen is not None:
+            assert (seen[..., 5] == float("inf")).all() and (seen[..., 38] == -float("inf")).all() and seen[..., 71].isnan().all()
+        assert (last[..., 5] == float("inf")).all() and last[..., 71].isnan().all()
+        assert last[..., 38].isnan().all() if t < S - 1 else (last[..., 38] == float("inf")).all()
+        touched = [5, 38, 71]
+    else:                                           # (groups of 32 channels are held as NaN)
+        seen = out[1, :4, t:]
+        assert seen[..., :96].isnan().all()
+        touched = range(96)
+    for c in touched:
+        out[1, :4, t:, c] = clean[1, :4, t:, c]
+    assert torch.equal(out, clean)
+
+
 def test_pools_past_4_gib(dev):
     """Byte offsets past 32 bits, element offsets past 31: the pages used are the last of a pool of 9000 pages of half a megabyte."""
     pages = alloc_pages(9000, 8, 256, "bf16")

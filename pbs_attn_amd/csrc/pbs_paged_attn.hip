@@ -422,6 +422,7 @@ struct Plan {
 };
 Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
+  max_len = std::min(max_len, PAGED_MAX_TOKENS);
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits == 4 ? 48 : rows <= 64 ? 64 : 128;
   // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512

@@ -65,6 +65,14 @@ def test_arguments_that_the_library_refuses():
         assert _read(lib, **change) == -1 and word in lib.pbs_last_error(), (change, lib.pbs_last_error())
 
 
+def test_a_workspace_does_not_grow_with_lengths_that_no_sequence_has():
+    size = _lib.load().pbs_paged_attn_workspace_bytes
+    for bits in (16, 4):
+        most = size(2, 8, 2, 1, 128, bits, 1 << 30)
+        assert 0 < most < 1 << 24 and size(2, 8, 2, 1, 128, bits, (1 << 31) - 1) == most
+        assert size(2, 8, 2, 1, 128, bits, 0) == size(2, 8, 2, 1, 128, bits, -1) == 0
+
+
 def test_pages_of_a_layer_have_one_of_two_forms():
     for form in ("bf16", "fp4"):
         for size in (32, 64, 128, 256):

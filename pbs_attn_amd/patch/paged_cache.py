@@ -89,6 +89,8 @@ class PagedKVCache(Cache):
 
     def lengths(self, n):
         """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same."""
+        if self.page_table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a paged cache's lengths are the host's and cannot be captured: capture ops.paged_append and ops.paged_attn")
         if n not in self._lengths:
             if len(self._lengths) >= 2:
                 del self._lengths[next(iter(self._lengths))]

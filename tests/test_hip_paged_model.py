@@ -73,3 +73,21 @@ def test_what_a_4_bit_cache_holds_of_a_prompt(dev):
     for b in range(2):
         for wide, narrow in zip(held[0][b], held[1][b]):
             assert torch.equal(narrow, held_in_4_bits(wide.to(torch.bfloat16)))
+
+
+def test_a_captured_step_keeps_lengths_of_its_own(dev):
+    """The cache's lengths are the host's: a graph would replay those of its capture, so there the cache refuses."""
+    from pbs_attn.patch.huggingface import get_paged_cache
+    from pbs_attn_amd.ttft import build_model
+    cache = get_paged_cache(build_model("llama31_8b", layers=1, device=dev), 1, 64)
+    x = torch.zeros(1, 8, 1, 128, dtype=torch.bfloat16, device=dev)
+    graph, y = torch.cuda.CUDAGraph(), torch.zeros(4, device=dev)
+    with torch.cuda.graph(graph):
+        y += 1
+        for call in (lambda: cache.layers[0].append(x, x), lambda: cache.update(x, x, 0)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    graph.replay()
+    assert cache.get_seq_length() == 0 and not cache._lengths
+    cache.update(x, x, 0)
+    assert cache.get_seq_length() == 1 and y.tolist() == [1.0] * 4

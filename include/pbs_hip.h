@@ -237,8 +237,8 @@ int pbs_rope_qk(const void* q, const void* k, const void* cos, const void* sin, 
                 int64_t k_ss, int64_t c_sb, int64_t c_ss, void* stream);
 
 /* A paged key-value cache.  A pool holds num_pages pages of page_size tokens (32, 64, 128 or 256) of Hkv heads; row b of page_table
- * ((B, max_pages) int32, row stride table_sb) lists the pages of sequence b in order, and token t of it lies in page t / page_size.  Only the
- * entries that a call's tokens reach are read; the tokens of an entry outside 0 .. num_pages - 1, and those behind max_pages, are not
+ * ((B, max_pages) int32, row stride table_sb) lists the pages of sequence b in order, and token t of it lies in page t / page_size.  Entries
+ * behind a sequence's tokens may hold anything; the tokens of an entry outside 0 .. num_pages - 1, and those behind max_pages, are not
  * stored, count as not there for the attention, and are read as zeros.
  *   kv_bits 16   k_pages (page, head, token, 128) bf16, v_pages (page, head, token / 8, 128, token % 8) bf16; no scales
  *   kv_bits 4    e2m1 codes, the even channel in a byte's low half: k_pages (page, head, token, 64 bytes), v_pages
@@ -267,6 +267,7 @@ int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale
 
 /* Attention of the new tokens (appended before) over their sequences: query row i < new_lens[b] of q (B, Hq, S, 128) sees the tokens
  * 0 .. past_lens[b] + i; out (B, Hq, S, 128) with its own strides.  Rows from new_lens[b] on, and rows whose keys weigh nothing, are zeros.
+ * What a row does not see does not reach it, infinities and NaN included.
  * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
  * positive.  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
 size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len);

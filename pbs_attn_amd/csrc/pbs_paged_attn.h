@@ -89,6 +89,8 @@ __device__ __forceinline__ void load_v(Tile<4>& t, const PagedPool& p, int64_t a
 
 // Values that are not finite, of tokens that some of a row tile's rows do not see (the call's own): not even times zero.  They leave the tile that
 // is multiplied, and the rows that see one get it at the end: what a row sees begins with the first token, so the first key is enough.
+// (Products of ones that count them instead, in registers, spilled.  Asked for by every row at the end, 35 rows take 64 us; only where one was
+// noted, 59.6; without any of it 57.8.)
 struct PagedLater {
   int up[PAGED_D], down[PAGED_D];   // by channel: the first key that is an infinity or NaN, for `up` all but -inf, for `down` all but +inf
   int any;

@@ -8,7 +8,7 @@
 // the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order and nothing is shared
 // but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
 // parts), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
-// 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 227 us (5.0).  35 rows in 4 bits are bound by the vector unit (58 us, 2.4 TB/s).
+// 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are bound by the vector unit (60 us, 2.3 TB/s).
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>

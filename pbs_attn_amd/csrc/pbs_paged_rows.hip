@@ -9,7 +9,7 @@
 // first beside the weights of the second.
 //
 // Bound by the matrix unit, and what keeps it from its rate is the softmax on the vector unit: 500 new tokens of two sequences behind up to 16k
-// (32 / 8 heads) 236 us, 890 TFLOP/s; 1000 behind 32k in 4 bits 577 us, 945 (without the order above 671, with the waits for the next
+// (32 / 8 heads) 241 us, 870 TFLOP/s; 1000 behind 32k in 4 bits 580 us, 940 (without the order above 671, with the waits for the next
 // tile's copies in front of each step's first product 700).  Of the time the matrix unit is busy half.
 #include "pbs_paged_attn.h"
 #include <math.h>

@@ -11,8 +11,11 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 constexpr int PAGED_WAVES = 4;       // of a workgroup
 constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences, at most: two a compute unit
-// A row's exponent is taken up where a logit is more than this above it (log2): weights stay below 2^8, which costs their sums in fp32 and their
-// roundings to bf16 nothing, and the sums are rescaled a few times in a sequence rather than with every new maximum.
+// A row's exponent m stays PAGED_ROOM .. PAGED_ROOM + PAGED_SLACK (log2) above its largest logit: it is taken up, by the most that it may be, where a
+// logit comes nearer, so the sums are rescaled a few times in a sequence rather than with every new maximum.  Weights are at most 2^-30, and there are at
+// most 2^30 tokens: the sums of weighted values, which are joined as they are, never pass the largest value that the cache holds, and stay finite as
+// their average does.  It costs the smallest numbers: weights of less than 2^-88 of the row's largest are zeros, values below 2^-88 lose bits.
+constexpr float PAGED_ROOM = 30.f;
 constexpr float PAGED_SLACK = 8.f;
 
 struct PagedHeader {   // of a worker: the piece of work that it began and left to the `more` workers after it

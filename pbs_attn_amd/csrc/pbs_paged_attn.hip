@@ -145,13 +145,13 @@ struct Softmax {
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], x[r][i][j]);
-      grows |= top[r] * c > m[r] + PAGED_SLACK;   // (this lane's keys; the row's are looked at where one of them is)
+      grows |= top[r] * c > m[r] - PAGED_ROOM;   // (this lane's keys; the row's are looked at where one of them is)
     }
     if (__any(grows)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float most = max_over_groups(top[r]) * c;
-        const float m_new = most > m[r] + PAGED_SLACK ? most : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
+        const float m_new = most > m[r] - PAGED_ROOM ? most + (PAGED_ROOM + PAGED_SLACK) : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;

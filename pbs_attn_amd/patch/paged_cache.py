@@ -79,6 +79,9 @@ class PagedKVCache(Cache):
             raise ValueError("a cache holds at least one sequence of at least one token")
         if page_size not in PAGE_SIZES:
             raise ValueError(f"pages of {PAGE_SIZES} tokens, got {page_size}")
+        kinds = getattr(config, "layer_types", None)
+        if any(kind != "full_attention" for kind in kinds) if kinds else getattr(config, "use_sliding_window", False):
+            raise ValueError("a layer on a paged cache attends to all that is cached, and this model has layers with sliding windows")
         heads = num_kv_heads or config.num_key_value_heads
         slots = (max_len + page_size - 1) // page_size
         self.sequences, self.room = batch_size, max_len

@@ -167,6 +167,10 @@ def patched_attention_forward(
         return self.original_forward(hidden_states=hidden_states, position_embeddings=position_embeddings,
                                      attention_mask=attention_mask, past_key_values=past_key_values,
                                      cache_position=cache_position, **kwargs)
+    if pages is not None and getattr(self, "first_patched", True):
+        # (a step's layers have the same mask)
+        from pbs_attn_amd.patch.paged_cache import check_mask
+        check_mask(attention_mask, pages.length, q_len)
 
     q, n_q = _split_heads(self.q_proj(hidden_states), bsz, q_len, self.head_dim)
     k, n_kv = _split_heads(self.k_proj(hidden_states), bsz, q_len, self.head_dim)
@@ -246,6 +250,7 @@ def apply_patch_with_prefill(model, prefill_fn: Optional[Callable] = None, skip_
             continue
         attn = layer.self_attn
         attn.original_forward = attn.forward
+        attn.first_patched = patched == 0
         attn.forward = types.MethodType(_make_forward(prefill_fn), attn)
         patched += 1
     print(f"Monkey patch applied. Patched {patched}/{len(layers)} layers.")

@@ -5,8 +5,8 @@ on the way.  The first prompt's attention is the prefill function's; single toke
 (``ops.paged_attn``), where the reference sends single tokens to the module's original forward and lets a later prompt attend to itself
 alone (pbs_attn/patch/huggingface.py:169-241).  Layers that are not patched (``skip_layers``) read their keys and values back (``update``).
 
-All sequences of a batch have one length, as the module's inputs have: there is no padding, and attention masks are not looked at (the
-prefill function takes none either).  The lengths are the host's: a program that captures its decoding step into a graph calls
+All sequences of a batch have one length, as the module's inputs have: there is no padding.  A mask that hides anything a causal one does not is
+refused (``check_mask``), and so are models with sliding windows.  The lengths are the host's: a program that captures its decoding step into a graph calls
 ``ops.paged_append`` and ``ops.paged_attn`` with lengths of its own on the GPU."""
 from __future__ import annotations
 
@@ -15,6 +15,29 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from pbs_attn_amd import ops
 from pbs_attn_amd.paged import HEAD_DIM, PAGE_SIZES, alloc_pages
+
+
+def check_mask(mask, past, new):
+    """Raises ValueError unless a module's attention mask says what the attention on a paged cache does: the first of ``new`` queries sees
+    ``past + 1`` keys, each one after it one more.  None says so, and a mask of (batch, keys) of ones, and one of (batch, heads, queries, keys)
+    that is causal, of truth values or added to the logits; columns behind the last key are not looked at.  Reads the mask on the host."""
+    if mask is None:
+        return
+    n = past + new
+    fits = False
+    if isinstance(mask, torch.Tensor) and mask.dim() in (2, 4) and mask.shape[-1] >= n:
+        if mask.dim() == 2:
+            fits = mask[:, :n].all()
+        elif mask.shape[2] == new:
+            fits = torch.ones((), dtype=torch.bool, device=mask.device)
+            keys = torch.arange(n, device=mask.device)
+            for i in range(0, new, 1024):       # (a prompt's mask is large)
+                rows = mask[:, :, i:i + 1024, :n]
+                seen = keys <= torch.arange(past + i, past + i + rows.shape[2], device=mask.device)[:, None]
+                same = rows == seen if rows.dtype == torch.bool else (rows == 0) == seen
+                fits &= same.all()
+    if not fits:
+        raise ValueError("a paged cache attends causally to all that is cached: no padding, windows or other masks")
 
 
 class _PagedLayer(CacheLayerMixin):

@@ -40,10 +40,31 @@ def check_mask(mask, past, new):
         raise ValueError("a paged cache attends causally to all that is cached: no padding, windows or other masks")
 
 
+class _Sequences:
+    """What the layers of a cache share: their number, the tokens that each has room for, their pages and lengths.  (It knows neither the
+    cache nor its layers: in a cycle the pages would stay until the collector's next pass.)"""
+
+    def __init__(self, count, room, page_size, device):
+        slots = (room + page_size - 1) // page_size
+        self.count, self.room = count, room
+        self.page_table = torch.arange(count * slots, dtype=torch.int32, device=device).view(count, slots)
+        self.kept = {}
+
+    def lengths(self, n):
+        """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same."""
+        if self.page_table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a paged cache's lengths are the host's and cannot be captured: capture ops.paged_append and ops.paged_attn")
+        if n not in self.kept:
+            if len(self.kept) >= 2:
+                del self.kept[next(iter(self.kept))]
+            self.kept[n] = torch.full((self.count,), n, dtype=torch.int32, device=self.page_table.device)
+        return self.kept[n]
+
+
 class _PagedLayer(CacheLayerMixin):
-    def __init__(self, cache, pages):
+    def __init__(self, sequences, pages):
         super().__init__()
-        self.cache, self.pages, self.length = cache, pages, 0
+        self.sequences, self.pages, self.length = sequences, pages, 0
         self.is_initialized = True
 
     def lazy_initialization(self, key_states, value_states):
@@ -51,23 +72,24 @@ class _PagedLayer(CacheLayerMixin):
 
     def append(self, k, v, **rotation):
         """New tokens k, v (batch, heads, S, 128) behind those that are there; the arguments and results of ``ops.paged_append``."""
-        if k.shape[0] != self.cache.sequences:
-            raise ValueError(f"a cache of {self.cache.sequences} sequences, {k.shape[0]} given")
-        if self.length + k.shape[2] > self.cache.room:
-            raise ValueError(f"{self.length} + {k.shape[2]} tokens, and the cache holds {self.cache.room}")
-        rotated = ops.paged_append(self.pages, self.cache.page_table, self.cache.lengths(self.length), k, v, **rotation)
+        s = self.sequences
+        if k.shape[0] != s.count:
+            raise ValueError(f"a cache of {s.count} sequences, {k.shape[0]} given")
+        if self.length + k.shape[2] > s.room:
+            raise ValueError(f"{self.length} + {k.shape[2]} tokens, and the cache holds {s.room}")
+        rotated = ops.paged_append(self.pages, s.page_table, s.lengths(self.length), k, v, **rotation)
         self.length += k.shape[2]
         return rotated
 
     def attention(self, q):
         """Of the last tokens, appended before: q (batch, heads, S, 128)."""
         past = self.length - q.shape[2]
-        return ops.paged_attn(q, self.pages, self.cache.page_table, self.cache.lengths(past), max_len=self.length)
+        return ops.paged_attn(q, self.pages, self.sequences.page_table, self.sequences.lengths(past), max_len=self.length)
 
     def update(self, key_states, value_states, *args, **kwargs):
         """For modules with an attention of their own: stores the (rotated) keys and the values, and returns all of them."""
         self.append(key_states, value_states)
-        return ops.paged_read(self.pages, self.cache.page_table, self.cache.lengths(self.length), self.length)
+        return ops.paged_read(self.pages, self.sequences.page_table, self.sequences.lengths(self.length), self.length)
 
     def get_mask_sizes(self, query_length, *args):
         return self.length + query_length, 0
@@ -76,7 +98,7 @@ class _PagedLayer(CacheLayerMixin):
         return self.length
 
     def get_max_length(self):
-        return self.cache.room
+        return self.sequences.room
 
     get_max_cache_shape = get_max_length
 
@@ -106,19 +128,15 @@ class PagedKVCache(Cache):
         if any(kind != "full_attention" for kind in kinds) if kinds else getattr(config, "use_sliding_window", False):
             raise ValueError("a layer on a paged cache attends to all that is cached, and this model has layers with sliding windows")
         heads = num_kv_heads or config.num_key_value_heads
-        slots = (max_len + page_size - 1) // page_size
-        self.sequences, self.room = batch_size, max_len
-        self.page_table = torch.arange(batch_size * slots, dtype=torch.int32, device=device).view(batch_size, slots)
-        self._lengths = {}
-        super().__init__(layers=[_PagedLayer(self, alloc_pages(batch_size * slots, heads, page_size, form, device))
+        self._shared = shared = _Sequences(batch_size, max_len, page_size, device)
+        super().__init__(layers=[_PagedLayer(shared, alloc_pages(shared.page_table.numel(), heads, page_size, form, device))
                                  for _ in range(config.num_hidden_layers)])
 
+    sequences = property(lambda self: self._shared.count)
+    room = property(lambda self: self._shared.room)
+    page_table = property(lambda self: self._shared.page_table)
+    _lengths = property(lambda self: self._shared.kept)
+
     def lengths(self, n):
-        """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same."""
-        if self.page_table.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a paged cache's lengths are the host's and cannot be captured: capture ops.paged_append and ops.paged_attn")
-        if n not in self._lengths:
-            if len(self._lengths) >= 2:
-                del self._lengths[next(iter(self._lengths))]
-            self._lengths[n] = torch.full((self.sequences,), n, dtype=torch.int32, device=self.page_table.device)
-        return self._lengths[n]
+        """``n`` for every sequence, on the GPU."""
+        return self._shared.lengths(n)

@@ -51,14 +51,19 @@ class _Sequences:
         self.kept = {}
 
     def lengths(self, n):
-        """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same."""
-        if self.page_table.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a paged cache's lengths are the host's and cannot be captured: capture ops.paged_append and ops.paged_attn")
-        if n not in self.kept:
+        """``n`` for every sequence, on the GPU; the last two are kept, as all layers of a step ask for the same.  A tensor is used on the
+        stream that filled it only: there its memory may be given away while the last call that reads it is still to come."""
+        stream = 0
+        if self.page_table.is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a paged cache's lengths are the host's and cannot be captured: capture ops.paged_append and ops.paged_attn")
+            stream = torch._C._cuda_getCurrentRawStream(self.page_table.device.index)
+        key = (n, stream)
+        if key not in self.kept:
             if len(self.kept) >= 2:
                 del self.kept[next(iter(self.kept))]
-            self.kept[n] = torch.full((self.count,), n, dtype=torch.int32, device=self.page_table.device)
-        return self.kept[n]
+            self.kept[key] = torch.full((self.count,), n, dtype=torch.int32, device=self.page_table.device)
+        return self.kept[key]
 
 
 class _PagedLayer(CacheLayerMixin):

@@ -110,8 +110,16 @@ class _PagedLayer(CacheLayerMixin):
     def reset(self):
         self.length = 0
 
+    def crop(self, tokens_to_remove):
+        """Takes that many tokens (negative: -3 for the last three) off the end; a positive number is how many stay, as the library's own
+        caches still have it."""
+        n = tokens_to_remove
+        self.length = max(self.length + n, 0) if n <= 0 else min(self.length, n)
+
     def reorder_cache(self, beam_idx):
-        raise NotImplementedError("a paged cache does not reorder its sequences")
+        raise NotImplementedError("a paged cache does not reorder, repeat or drop its sequences")
+
+    batch_select_indices = batch_repeat_interleave = reorder_cache
 
 
 class PagedKVCache(Cache):

@@ -120,9 +120,11 @@ def get_permuted_block_sparse_attn_fwd(
 
 def get_paged_cache(model, batch_size, max_len, page_size=64, form="bf16"):
     """A ``PagedKVCache`` (pbs_attn_amd/patch/paged_cache.py) for a model whose layers are patched: pass it as ``past_key_values``.  ``form``:
-    "bf16", or "fp4" for 4 bits."""
+    "bf16", or "fp4" for 4 bits.  All layers are on one device."""
     from pbs_attn_amd.patch.paged_cache import PagedKVCache
     k_proj = model.model.layers[0].self_attn.k_proj
+    if any(layer.self_attn.k_proj.weight.device != k_proj.weight.device for layer in model.model.layers):
+        raise ValueError("a paged cache lies on one device, and this model's layers do not")
     head_dim = getattr(model.config, "head_dim", None) or model.config.hidden_size // model.config.num_attention_heads
     return PagedKVCache(model.config, batch_size, max_len, page_size, form, k_proj.weight.device, k_proj.weight.shape[0] // head_dim)
 

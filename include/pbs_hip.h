@@ -24,7 +24,8 @@
 extern "C" {
 #endif
 
-int pbs_abi_version(void);
+#define PBS_ABI_VERSION 1   /* goes up where a declaration below changes */
+int pbs_abi_version(void);   /* the library's */
 const char* pbs_last_error(void);
 
 /* Key scoring: scores[b,h,k] = mean over the last 128 queries of

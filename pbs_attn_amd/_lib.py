@@ -128,6 +128,9 @@ def paged_host():
             spec = importlib.util.spec_from_file_location("_pbs_paged", PAGED_HOST_PATH)
             host = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(host)
+            built_for, here = (getattr(host, "torch_version", None), getattr(host, "abi_version", None)), (str(torch.__version__), lib.pbs_abi_version())
+            if built_for != here:
+                raise ImportError(f"built for torch and library {built_for}, not {here}")
         except ImportError as e:
             import warnings
             _paged_host = _no_paged_host

@@ -84,7 +84,7 @@ def build_paged_host_module() -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + sysconfig.get_path("include"),
                     "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", PAGED_HOST_SRC, "-o", PAGED_HOST_PATH,
+                    f'-DPBS_TORCH_VERSION="{torch.__version__}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", PAGED_HOST_SRC, "-o", PAGED_HOST_PATH,
                     "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], check=True)
     return PAGED_HOST_PATH
 

@@ -47,7 +47,7 @@ int pbs_require_no_static_lds(const void* kernel, const char* what) {
   return 0;
 }
 
-extern "C" int pbs_abi_version(void) { return 1; }
+extern "C" int pbs_abi_version(void) { return PBS_ABI_VERSION; }
 
 namespace {
 

@@ -2,7 +2,8 @@
 //
 // A decoding step's calls take the GPU 3 to 12 us, and reading eight to twelve tensors in Python takes longer: the next token of a chat into
 // the cache 17.1 us a call in Python, 6.5 here.  Tensors are read through torch's C++ interface here (an attribute read through Python takes 0.1 us, and a
-// call reads fifty), so the module is built for one interpreter and one torch; where it is missing the calls go through Python.
+// call reads fifty), so the module is built for one interpreter and one torch, and says which: with another one, or without the module, the calls go
+// through Python.
 //
 // Whatever is not the plain case returns None with nothing done, and the general path in Python takes the call, or refuses it with its message.
 #define PY_SSIZE_T_CLEAN
@@ -268,5 +269,8 @@ PyMODINIT_FUNC PyInit__pbs_paged() {
   s_v = PyUnicode_InternFromString("v");
   s_k_scale = PyUnicode_InternFromString("k_scale");
   s_v_scale = PyUnicode_InternFromString("v_scale");
-  return s_k && s_v && s_k_scale && s_v_scale ? PyModule_Create(&module) : nullptr;
+  PyObject* m = s_k && s_v && s_k_scale && s_v_scale ? PyModule_Create(&module) : nullptr;
+  if (m && !PyModule_AddStringConstant(m, "torch_version", PBS_TORCH_VERSION) && !PyModule_AddIntConstant(m, "abi_version", PBS_ABI_VERSION)) return m;
+  Py_XDECREF(m);
+  return nullptr;
 }

@@ -155,10 +155,13 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (q) q_out = at::empty({B, Hq, S, HEAD_DIM}, q->options());
   if (args[9] == Py_True) k_out = at::empty({B, Hkv, S, HEAD_DIM}, k->options());
   const auto address = [](const at::Tensor* t) { return t ? t->const_data_ptr() : nullptr; };
+  // (written: a lazy copy becomes a copy here)
+  void *kp = pages.k.mutable_data_ptr(), *vp = pages.v.mutable_data_ptr();
+  void *ksp = pages.k_scale.defined() ? pages.k_scale.mutable_data_ptr() : nullptr, *vsp = pages.v_scale.defined() ? pages.v_scale.mutable_data_ptr() : nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = append_fn(address(q), address(k), address(v), address(cos), address(sin), q ? q_out.mutable_data_ptr() : nullptr,
-                 k_out.defined() ? k_out.mutable_data_ptr() : nullptr, (void*)pages.kp(), (void*)pages.vp(), (void*)pages.ksp(), (void*)pages.vsp(),
+                 k_out.defined() ? k_out.mutable_data_ptr() : nullptr, kp, vp, ksp, vsp,
                  (const int32_t*)address(table), (const int32_t*)address(past), (const int32_t*)address(fresh), (int)B, (int)Hq, (int)Hkv, (int)S, HEAD_DIM,
                  (int)pages.n, (int)table->size(1), (int)pages.size, pages.bits(), q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? q->stride(2) : 0,
                  k->stride(0), k->stride(1), k->stride(2), v->stride(0), v->stride(1), v->stride(2), cos && cos->size(0) > 1 ? cos->stride(0) : 0,

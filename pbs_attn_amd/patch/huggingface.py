@@ -172,7 +172,12 @@ def patched_attention_forward(
     if pages is not None and getattr(self, "first_patched", True):
         # (a step's layers have the same mask)
         from pbs_attn_amd.patch.paged_cache import check_mask
-        check_mask(attention_mask, pages.length, q_len)
+        try:
+            check_mask(attention_mask, pages.length, q_len)
+        except ValueError:
+            for layer in past_key_values.layers:     # (layers ahead that are not patched have stored the tokens)
+                layer.length = min(layer.length, pages.length)
+            raise
 
     q, n_q = _split_heads(self.q_proj(hidden_states), bsz, q_len, self.head_dim)
     k, n_kv = _split_heads(self.k_proj(hidden_states), bsz, q_len, self.head_dim)

@@ -175,7 +175,8 @@ struct ReadArgs {
   int L;
 };
 
-// A workgroup per tile of 32 tokens and head, K and V.  Bound by memory (18 000 tokens of 4 heads out of 4 bits: 47 MB in 10 us).
+// A workgroup per tile of 32 tokens and head, K and V.  Bound by memory (18 000 tokens of 4 heads out of 4 bits: 47 MB in 9 us;
+// out of bf16: 74 MB in 13.5 us).
 template <int BITS>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const int tile = blockIdx.x, h = blockIdx.y, b = blockIdx.z;

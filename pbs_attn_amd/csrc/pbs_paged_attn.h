@@ -14,7 +14,8 @@ constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequenc
 // A row's exponent m stays PAGED_ROOM .. PAGED_ROOM + PAGED_SLACK (log2) above its largest logit: it is taken up, by the most that it may be, where a
 // logit comes nearer, so the sums are rescaled a few times in a sequence rather than with every new maximum.  Weights are at most 2^-30, and there are at
 // most 2^30 tokens: the sums of weighted values, which are joined as they are, never pass the largest value that the cache holds, and stay finite as
-// their average does.  It costs the smallest numbers: weights of less than 2^-88 of the row's largest are zeros, values below 2^-88 lose bits.
+// their average does (with logits below 2^24; above, the exponent itself is rounded).  It costs the smallest numbers: weights of less than 2^-88
+// of the row's largest are zeros, and values below 2^-88 lose bits.
 constexpr float PAGED_ROOM = 30.f;
 constexpr float PAGED_SLACK = 8.f;
 

@@ -8,7 +8,9 @@
 // the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order and nothing is shared
 // but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
 // parts), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
-// 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are bound by the vector unit (60 us, 2.3 TB/s).
+// 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their
+// time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 12 registers of a wave
+// go to scratch memory, 13 with eight waves.)
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>
@@ -165,7 +167,7 @@ struct Softmax {
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        // half a step of 2^-8 off, above the line and below it
+        // bf16, as the matrix instruction takes them: half a step is 2^-8 of a weight, above the line and below it
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i][j], c, -m[r]));
         l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i], l[r], 0, 0, 0);
@@ -426,7 +428,9 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits == 4 ? 48 : rows <= 64 ? 64 : 128;
   // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512
-  // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.
+  // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.  Many sequences of 700 tokens in
+  // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
+  // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
   const bool cut = max_len > (kv_bits == 16 ? 640 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // (no more workers than there is work for)
@@ -495,7 +499,9 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   }
   if (p.workers) {
     const int rows = (int)std::min<int64_t>(p.rows, (int64_t)S * a.G);
-    // (parts of a row, if sequences are alike: with 32 heads' rows of one sequence, 4 KV heads, 128)
+    // (parts of a row, if sequences are alike: with 32 heads' rows of one sequence, 4 KV heads, 128.  Where they are not, a long one's parts are
+    // joined by fewer groups than they could be: one of 100000 tokens among 63 of 500, 8 KV heads, bf16 109 us, 4 bits 48, of which the cache
+    // takes 109 and 29 at a copy's rate.)
     const int64_t parts = p.workers / units;
     if (parts >= 32) hipLaunchKernelGGL(join_kernel<16>, dim3(p.workers, rows), dim3(256), 0, st, a, p.rows);
     else if (parts >= 4) hipLaunchKernelGGL(join_kernel<4>, dim3(p.workers, (rows + 3) / 4), dim3(256), 0, st, a, p.rows);

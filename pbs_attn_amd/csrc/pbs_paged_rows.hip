@@ -8,9 +8,10 @@
 // A wave's order within a step keeps both units busy: the logits of its second 32 keys beside the weights of the first, the products of the
 // first beside the weights of the second.
 //
-// Bound by the matrix unit, and what keeps it from its rate is the softmax on the vector unit: 500 new tokens of two sequences behind up to 16k
-// (32 / 8 heads) 241 us, 870 TFLOP/s; 1000 behind 32k in 4 bits 580 us, 940 (without the order above 671, with the waits for the next
-// tile's copies in front of each step's first product 700).  Of the time the matrix unit is busy half.
+// 500 new tokens of two sequences behind up to 16k (32 / 8 heads) 241 us, 870 TFLOP/s; 1000 behind 32k in 4 bits 582 us, 940 (without the order
+// above 671, with the waits for the next tile's copies in front of each step's first product 700).  By the counters neither unit is full: in bf16
+// the matrix unit works 49 % of the time and the vector unit 49 %, in 4 bits 43 and 55; two waves a SIMD with 32 rows each overlap them no
+// further.  (In 4 bits two registers of a wave go to scratch memory.)
 #include "pbs_paged_attn.h"
 #include <math.h>
 
@@ -232,7 +233,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       }
     };
     auto weigh = [&](int r, int i) __attribute__((always_inline)) {
-      // half a step of 2^-8 off, above the line and below it
+      // bf16, as the matrix instruction takes them: half a step is 2^-8 of a weight, above the line and below it
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i][j & 1][j >> 1], c, -m[r]));
     };

@@ -270,7 +270,7 @@ int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale
  * 0 .. past_lens[b] + i; out (B, Hq, S, 128) with its own strides.  Rows from new_lens[b] on, and rows whose keys weigh nothing, are zeros.
  * What a row does not see does not reach it, infinities and NaN included.  Logits, sums and the largest exponent are fp32; the weights that
  * multiply the values are rounded to bf16 (2^-8 of each at most), and what divides is the sum of the rounded ones.  Finite logits and values give
- * finite results, up to the largest; values below 2^-88 lose bits.
+ * finite results, up to the largest; the smallest (with room for 2^17 tokens in the table, values below 2^-116) lose bits.
  * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
  * positive.  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
 size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len);

@@ -11,12 +11,11 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 constexpr int PAGED_WAVES = 4;       // of a workgroup
 constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences, at most: two a compute unit
-// A row's exponent m stays PAGED_ROOM .. PAGED_ROOM + PAGED_SLACK (log2) above its largest logit: it is taken up, by the most that it may be, where a
-// logit comes nearer, so the sums are rescaled a few times in a sequence rather than with every new maximum.  Weights are at most 2^-30, and there are at
-// most 2^30 tokens: the sums of weighted values, which are joined as they are, never pass the largest value that the cache holds, and stay finite as
-// their average does (with logits below 2^24; above, the exponent itself is rounded).  It costs the smallest numbers: weights of less than 2^-88
-// of the row's largest are zeros, and values below 2^-88 lose bits.
-constexpr float PAGED_ROOM = 30.f;
+// A row's exponent m stays `room` .. `room` + PAGED_SLACK (log2) above its largest logit: it is taken up, by the most that it may be, where a logit
+// comes nearer, so the sums are rescaled a few times in a sequence rather than with every new maximum.  2^room is as many tokens as the table has
+// room for, so the sums of weighted values, which are joined as they are, never pass the largest value that the cache holds, and stay finite as
+// their average does (with logits below 2^24; above, the exponent itself is rounded).  It costs the smallest numbers, which come nearer to fp32's
+// least, 2^-149: with room for 2^17 tokens weights of less than 2^-101 of the row's largest are zeros, and values below 2^-116 lose bits.
 constexpr float PAGED_SLACK = 8.f;
 
 struct PagedHeader {   // of a worker: the piece of work that it began and left to the `more` workers after it
@@ -34,6 +33,7 @@ struct PagedAttnArgs {
   int B, Hq, Hkv, S, G, row_tiles, workers;
   int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
   float scale_log2;   // softmax scale times log2(e)
+  float room;
 };
 
 // a slot: rows of 128 sums, then each row's largest exponent and sum of weights

@@ -9,8 +9,8 @@
 // but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
 // parts), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
 // 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their
-// time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 12 registers of a wave
-// go to scratch memory, 13 with eight waves.)
+// time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 13 registers of a wave
+// go to scratch memory, 20 with eight waves.)
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>
@@ -119,7 +119,7 @@ struct Softmax {
   }
   // logits of the NT tiles; `k0`: the first one's first key, `keys`: how many there are, bit i of `gone`: tile i's page is not there
   template <bool MASK>
-  __device__ __forceinline__ void weigh(const Tile<BITS> (&t)[NT], bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, float c, int n, int g) {
+  __device__ __forceinline__ void weigh(const Tile<BITS> (&t)[NT], bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, float c, float room, int n, int g) {
     if (R > 1) asm volatile("" ::: "memory");   // (or all queries are read ahead of the loop, into registers)
     // (all row tiles' products first, then one decision: nothing waits for a row tile's maximum)
     float x[R][NT][8], top[R];
@@ -147,13 +147,13 @@ struct Softmax {
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top[r] = fmaxf(top[r], x[r][i][j]);
-      grows |= top[r] * c > m[r] - PAGED_ROOM;   // (this lane's keys; the row's are looked at where one of them is)
+      grows |= __builtin_fmaf(top[r], c, room) > m[r];   // (this lane's keys; the row's are looked at where one of them is)
     }
     if (__any(grows)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float most = max_over_groups(top[r]) * c;
-        const float m_new = most > m[r] - PAGED_ROOM ? most + (PAGED_ROOM + PAGED_SLACK) : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
+        const float m_new = most + room > m[r] ? most + (room + PAGED_SLACK) : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= f;
@@ -239,7 +239,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     uint32_t gone_next = 0;
     if (load) gone_next = look_up(R == 1 || next < end ? next : t);
     bf16x8 p[R][NT];
-    s.template weigh<mask.value>(tile, p, k0, u.keys, gone, a.scale_log2, n, g);
+    s.template weigh<mask.value>(tile, p, k0, u.keys, gone, a.scale_log2, a.room, n, g);
     if (load) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
@@ -477,6 +477,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.S = S; a.G = Hq / Hkv;
   a.q_sb = q_sb; a.q_sh = q_sh; a.q_ss = q_ss; a.o_sb = o_sb; a.o_sh = o_sh; a.o_ss = o_ss;
   a.scale_log2 = softmax_scale * 1.44269504088896340736f;
+  a.room = (float)(32 - __builtin_clz((unsigned)(max_pages * page_size - 1)));   // (32 tokens at least)
   a.row_tiles = (S * a.G + p.rows - 1) / p.rows;
   const int64_t units = (int64_t)B * Hkv * a.row_tiles;
   PBS_REQUIRE(units < (1 << 22), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)

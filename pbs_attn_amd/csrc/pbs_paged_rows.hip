@@ -11,7 +11,7 @@
 // 500 new tokens of two sequences behind up to 16k (32 / 8 heads) 241 us, 870 TFLOP/s; 1000 behind 32k in 4 bits 582 us, 940 (without the order
 // above 671, with the waits for the next tile's copies in front of each step's first product 700).  By the counters neither unit is full: in bf16
 // the matrix unit works 49 % of the time and the vector unit 49 %, in 4 bits 43 and 55; two waves a SIMD with 32 rows each overlap them no
-// further.  (In 4 bits two registers of a wave go to scratch memory.)
+// further.
 #include "pbs_paged_attn.h"
 #include <math.h>
 
@@ -256,13 +256,13 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         top[r] = s[r][i][0][0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top[r] = fmaxf(top[r], s[r][i][j & 1][j >> 1]);
-        grows |= top[r] * c > m[r] - PAGED_ROOM;   // (this lane's keys; the row's are looked at where one of them is)
+        grows |= __builtin_fmaf(top[r], c, a.room) > m[r];   // (this lane's keys; the row's are looked at where one of them is)
       }
       if (__any(grows)) {
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
           const float most = max_over_groups(top[r]) * c;
-          const float m_new = most > m[r] - PAGED_ROOM ? most + (PAGED_ROOM + PAGED_SLACK) : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
+          const float m_new = most + a.room > m[r] ? most + (a.room + PAGED_SLACK) : m[r], f = __builtin_amdgcn_exp2f(m[r] - m_new);   // (a row goes by its own keys)
           l[r] *= f;
 #pragma unroll
           for (int d = 0; d < 8; ++d) o[r][d] *= f;

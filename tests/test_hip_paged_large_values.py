@@ -62,3 +62,12 @@ def test_small_values(dev, form, S, total):
     k, q = _randn(g, 1, 2, total, 128) * 0.1, _randn(g, 1, 8, S, 128)
     v = (_randn(g, 1, 2, total, 128).float() * 2.0 ** -84).to(torch.bfloat16)
     _check(form, S, total, k, v, q, 2.0 ** 84)
+
+
+@pytest.mark.parametrize("form,down", [("bf16", 109), ("bf16", 104), ("fp4", 99)])      # (4 bits: groups of less than 2^-100 are not held exactly)
+@pytest.mark.parametrize("S,total", SIZES)
+def test_the_smallest_values(dev, form, down, S, total):
+    g = torch.Generator(device="cuda").manual_seed(S)
+    k, q = _randn(g, 1, 2, total, 128) * 0.1, _randn(g, 1, 8, S, 128)
+    v = (_randn(g, 1, 2, total, 128).float() * 2.0 ** -down).to(torch.bfloat16)
+    _check(form, S, total, k, v, q, 2.0 ** down)

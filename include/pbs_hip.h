@@ -242,6 +242,11 @@ int pbs_rope_qk(const void* q, const void* k, const void* cos, const void* sin, 
  * behind a sequence's tokens may hold anything; the tokens of an entry outside 0 .. num_pages - 1, and those behind max_pages, are not
  * stored, count as not there for the attention, and are read as zeros.
  *   kv_bits 16   k_pages (page, head, token, 128) bf16, v_pages (page, head, token / 8, 128, token % 8) bf16; no scales
+ *   kv_bits 8    e4m3 codes in the layouts of 16 bits; k_scale, v_scale (page, head, token / 32) bytes: the exponent of the power of two that
+ *                the codes of 32 tokens of a head (positions 32 t .. 32 t + 31 of a sequence) are multiplied by, plus 127.  The smallest
+ *                exponent is taken with which no finite value is above 448 units, within -100 .. 119, larger magnitudes being held as
+ *                448 * 2^119; an infinity or NaN is held as NaN.  Tokens that join others may take their exponent up, never down:
+ *                the codes that are there are then divided by the same power of two and rounded to nearest even once more.
  *   kv_bits 4    e2m1 codes, the even channel in a byte's low half: k_pages (page, head, token, 64 bytes), v_pages
  *                (page, head, token / 4, channel / 8, token % 4, 4 bytes); k_scale, v_scale (page, head, token / 32, channel / 32, token % 32)
  *                bytes: the exponent of the power of two that the group's codes are multiples of, plus 127.  The smallest exponent is

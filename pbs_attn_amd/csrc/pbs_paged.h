@@ -1,9 +1,11 @@
-// The pages of a key-value cache: layout, addresses and the 4-bit form, shared by the kernels that write, read and attend to them.
+// The pages of a key-value cache: layout, addresses and the 8- and 4-bit forms, shared by the kernels that write, read and attend to them.
 //
 // A page holds `page_size` tokens (32, 64, 128 or 256) of every KV head, head-major, so what a wave reads of one head is contiguous.
 //   bf16   K (page, head, token, 128)                       a token's row, as the caller has it
 //          V (page, head, token / 8, 128, token % 8)        eight tokens of a channel in 16 bytes: the matrix instruction's operand
 //                                                           of V^T, loaded from memory into registers without a transposition
+//   8 bits K (page, head, token, 128 bytes), V (page, head, token / 8, 128, token % 8 bytes): as in bf16
+//          scales of K and V (page, head, token / 32): one byte for the 32 tokens of a tile and head
 //   4 bits K (page, head, token, 64 bytes)                  channel 2j in the low half of byte j
 //          V (page, head, token / 4, 16, token % 4, 4 bytes) channels 8m .. 8m + 7 of four tokens in 16 bytes
 //          scales of K and V (page, head, token / 32, 4, token % 32): one byte a token and group of 32 channels
@@ -11,6 +13,10 @@
 // 4 bits: e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times 2^e, e + 127 in the byte.  e is the smallest exponent with no
 // value of the group above 7 * 2^e: then none is off by more than half the largest step (7 itself becomes 6).  -100 <= e <= 125:
 // smaller groups are held as zeros, and 6 * 2^125 is the largest value held.  A group with an infinity or NaN is held as NaN (byte 255).
+// 8 bits: e4m3 values (4 bits of precision, up to 448, multiples of 2^-9) times 2^e, e + 127 in the byte.  e is the smallest exponent with no
+// finite value of the tile above 448 * 2^e, -100 <= e <= 119; 448 * 2^119 is the largest value held.  An infinity or NaN is held as NaN, by itself.
+// The tile's exponent goes up with the tokens that join it, and the codes that are there follow (which rounds those that become less than
+// 2^-6 of the scale once more); it starts anew with the tile's first token and never goes down, also where tokens come off the sequence's end.
 // Scales are powers of two and the conversions round to nearest even, so what is held follows from the bf16 values alone, to the bit.
 #pragma once
 #include "pbs_common.h"
@@ -22,7 +28,7 @@ constexpr int PAGED_MAX_TOKENS = 1 << 30;   // of a sequence: positions stay in 
 struct PagedPool {
   char* k;
   char* v;
-  uint8_t* ks;   // scales, 4 bits only
+  uint8_t* ks;   // scales, 8 and 4 bits only
   uint8_t* vs;
   const int32_t* table;   // (B, max_pages)
   int64_t table_sb;
@@ -67,6 +73,35 @@ __device__ __forceinline__ u32x4 fp4_values(uint32_t codes, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
+// ---- 8 bits ----------------------------------------------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(2))) short s16x2;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+constexpr uint32_t FP8_MOST = 0x7f60u;   // 448 * 2^119 in bf16
+__device__ __forceinline__ bool not_finite(uint32_t bf16_bits) { return (bf16_bits & 0x7f80u) == 0x7f80u; }
+__device__ __forceinline__ bool fp8_is_nan(uint32_t code) { return (code & 0x7fu) == 0x7fu; }
+
+// scale byte of a tile whose largest finite magnitude has these bits (bf16, no sign)
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax) {
+  return (uint32_t)min(max((int)((amax + 0x1fu) >> 7) - 8, 27), 246);   // the exponent field, one up where the value is above 1.75 * 2^n
+}
+// two bf16 values with what the conversion does not take mended: infinities become NaN, larger magnitudes 448 * 2^119
+__device__ __forceinline__ uint32_t fp8_ready(uint32_t x) {
+  auto one = [](uint32_t h) { return not_finite(h) ? h | 0x40u : (h & 0x8000u) | min(h & 0x7fffu, FP8_MOST); };
+  return one(x & 0xffffu) | (one(x >> 16) << 16);
+}
+// 4 bf16 values (two a word) -> 4 codes; `scale` = 2^e.  (Divides by the scale and rounds to nearest even.)
+__device__ __forceinline__ uint32_t fp8_codes(uint32_t a, uint32_t b, float scale) {
+  s16x2 r = {};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, a), scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, b), scale, 1);
+  return __builtin_bit_cast(uint32_t, r);
+}
+// the values of codes 2 HIGH and 2 HIGH + 1 of a word, bf16 (exact: 4 bits times a power of two in the range above)
+template <int HIGH>
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
 }
 
 // checks that every entry point on pages makes; fills `p`

@@ -6,7 +6,8 @@ int paged_pool(PagedPool* p, const char* what, const void* k_pages, const void* 
                const int32_t* page_table, int64_t table_sb, int B, int Hkv, int head_dim, int num_pages, int max_pages, int page_size, int kv_bits) {
   PBS_REQUIRE(k_pages && v_pages && page_table, "%s: null tensor pointer", what);
   PBS_REQUIRE(head_dim == PAGED_D, "%s: head_dim must be 128, got %d", what, head_dim);
-  PBS_REQUIRE(kv_bits == 16 || kv_bits == 4, "%s: a cache of 16 or 4 bits, got %d", what, kv_bits);
+  PBS_REQUIRE(kv_bits == 16 || kv_bits == 4 || (kv_bits == 8 && k_scale && v_scale), "%s: a cache of 16 or 4 bits, or of 8 with its scales, got %d", what,
+              kv_bits);
   PBS_REQUIRE(kv_bits == 16 || (k_scale && v_scale), "%s: a cache of 4 bits needs its scales", what);
   PBS_REQUIRE(page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "%s: pages of 32, 64, 128 or 256 tokens, got %d", what, page_size);
   PBS_REQUIRE(B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535, "%s: bad shape", what);
@@ -45,6 +46,19 @@ __device__ __forceinline__ uint32_t largest_bits(u32x4 x) {
   return m;
 }
 
+__device__ __forceinline__ uint32_t largest_finite_bits(uint32_t x) {
+  const uint32_t lo = x & 0x7fffu, hi = (x >> 16) & 0x7fffu;
+  return max(not_finite(lo) ? 0u : lo, not_finite(hi) ? 0u : hi);
+}
+// the largest over the workgroup
+__device__ __forceinline__ uint32_t max_of_group(uint32_t m, uint32_t (&lds)[4]) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+}
+
 // x c - y s, x and y c + x s of bf16 pairs: the products are exact in fp32, the sum is rounded once to fp32 and the result once to bf16
 __device__ __forceinline__ uint32_t rotate_pair(uint32_t x, uint32_t y, uint32_t c, uint32_t s, float sign) {
   const float lo = __builtin_fmaf(sign * bf16_bits_to_f32(y & 0xffffu), bf16_bits_to_f32(s & 0xffffu), bf16_bits_to_f32(x & 0xffffu) * bf16_bits_to_f32(c & 0xffffu));
@@ -71,6 +85,41 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int c = threadIdx.x & 7, row = threadIdx.x >> 3, s = first + row;
   const bool in_call = s >= 0 && s < a.S, stored = s >= 0 && s < fresh;
 
+  if (kind == 2 && BITS == 8) {
+    // eight tokens of two channels, as in bf16: a lane's 16 bytes of the cache, which may hold tokens from before the call
+    __shared__ uint32_t most[4];
+    if (fresh == 0) return;
+    const int64_t at = paged_tile_index(a.pool, b, h0, tile);
+    if (at < 0) return;
+    const int d = (threadIdx.x & 63) * 2, s0 = first + (threadIdx.x >> 6) * 8;
+    const uint16_t* src = a.v + b * a.v_sb + h0 * a.v_sh + d;
+    u32x4* dst = (u32x4*)(a.pool.v + at * paged_tile_bytes<8>()) + threadIdx.x;
+    const uint32_t e_old = first < 0 ? a.pool.vs[at] : 0;
+    u32x4 x = {};
+    if (s0 < 0 || (s0 < fresh && s0 + 8 > fresh)) x = *dst;
+    uint32_t w[8], m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = s0 + j >= 0 && s0 + j < fresh ? *(const uint32_t*)(src + (int64_t)(s0 + j) * a.v_ss) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, largest_finite_bits(w[j]));
+    const uint32_t e = max(e_old, fp8_scale_byte(max_of_group(m, most)));
+    const float scale = __uint_as_float(e << 23), was = __uint_as_float(e_old << 23);
+#pragma unroll
+    for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t pick = c2 ? 0x07060302u : 0x05040100u;
+        const uint32_t y = fp8_codes(fp8_ready(__builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], pick)), fp8_ready(__builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], pick)), scale);
+        uint32_t old = x[2 * c2 + q], mine = 0;
+        if (e != e_old && s0 < 0) old = fp8_codes(fp8_pair<0>(old, was), fp8_pair<1>(old, was), scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine |= s0 + 4 * q + j >= 0 && s0 + 4 * q + j < fresh ? 0xffu << (8 * j) : 0u;
+        x[2 * c2 + q] = (y & mine) | (old & ~mine);
+      }
+    if ((s0 + 8 > 0 && s0 < fresh) || (s0 < 0 && e != e_old)) *dst = x;
+    if (threadIdx.x == 0 && e != e_old) a.pool.vs[at] = (uint8_t)e;
+    return;
+  }
   if (kind == 2 && BITS == 16) {
     // eight tokens of two channels: rows are read whole (a wave reads 256 bytes of each), the cache gets 32 bytes a lane
     const int d = (threadIdx.x & 63) * 2, eight = threadIdx.x >> 6, s0 = first + eight * 8;
@@ -139,7 +188,42 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       if (kind == 0) continue;
     }
     const int64_t at = paged_tile_index(a.pool, b, h, tile);
-    if (BITS == 16) {   // K
+    if (BITS == 8) {   // K; rows of the tile that were there before the call are this thread's too
+      __shared__ uint32_t most[4];
+      if (at < 0 || first >= fresh || fresh == 0) return;
+      char* dst = a.pool.k + at * paged_tile_bytes<8>() + row * PAGED_D + c * 8;
+      const uint32_t e_old = first < 0 ? a.pool.ks[at] : 0;
+      u32x2 y0 = {}, y1 = {};
+      if (s < 0) {
+        y0 = *(const u32x2*)dst;
+        y1 = *(const u32x2*)(dst + 64);
+      }
+      uint32_t m = 0;
+      if (stored) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, max(largest_finite_bits(x0[i]), largest_finite_bits(x1[i])));
+      }
+      const uint32_t e = max(e_old, fp8_scale_byte(max_of_group(m, most)));
+      const float scale = __uint_as_float(e << 23), was = __uint_as_float(e_old << 23);
+      if (s < 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          y0[i] = fp8_codes(fp8_pair<0>(y0[i], was), fp8_pair<1>(y0[i], was), scale);
+          y1[i] = fp8_codes(fp8_pair<0>(y1[i], was), fp8_pair<1>(y1[i], was), scale);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          y0[i] = fp8_codes(fp8_ready(x0[2 * i]), fp8_ready(x0[2 * i + 1]), scale);
+          y1[i] = fp8_codes(fp8_ready(x1[2 * i]), fp8_ready(x1[2 * i + 1]), scale);
+        }
+      }
+      if (stored || (s < 0 && e != e_old)) {
+        *(u32x2*)dst = y0;
+        *(u32x2*)(dst + 64) = y1;
+      }
+      if (threadIdx.x == 0 && e != e_old) a.pool.ks[at] = (uint8_t)e;
+    } else if (BITS == 16) {   // K
       if (at >= 0 && stored) {
         uint16_t* dst = (uint16_t*)(a.pool.k + at * paged_tile_bytes<16>()) + row * PAGED_D + c * 8;
         *(u32x4*)dst = x0;
@@ -186,7 +270,37 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const int64_t out = (((int64_t)b * a.pool.heads + h) * a.L + tile * PAGED_TILE) * PAGED_D;
   const int c = threadIdx.x & 7, row = threadIdx.x >> 3;
   const bool held = at >= 0 && row < len;
-  if (BITS == 16) {
+  if (BITS == 8) {
+    u32x4 x0 = {}, x1 = {};
+    if (held) {
+      const char* src = a.pool.k + at * paged_tile_bytes<8>() + row * PAGED_D + c * 8;
+      const float scale = __uint_as_float((uint32_t)a.pool.ks[at] << 23);
+      const u32x2 y0 = *(const u32x2*)src, y1 = *(const u32x2*)(src + 64);
+      x0 = (u32x4){fp8_pair<0>(y0[0], scale), fp8_pair<1>(y0[0], scale), fp8_pair<0>(y0[1], scale), fp8_pair<1>(y0[1], scale)};
+      x1 = (u32x4){fp8_pair<0>(y1[0], scale), fp8_pair<1>(y1[0], scale), fp8_pair<0>(y1[1], scale), fp8_pair<1>(y1[1], scale)};
+    }
+    if (row < rows) {
+      uint16_t* dst = a.k_out + out + row * PAGED_D + c * 8;
+      *(u32x4*)dst = x0;
+      *(u32x4*)(dst + 64) = x1;
+    }
+    const int d = (threadIdx.x & 63) * 2, eight = threadIdx.x >> 6;   // eight tokens of two channels
+    uint32_t y0[4] = {}, y1[4] = {};   // two tokens of a channel each
+    if (at >= 0 && eight * 8 < len) {
+      const u32x4 y = *((const u32x4*)(a.pool.v + at * paged_tile_bytes<8>()) + threadIdx.x);
+      const float scale = __uint_as_float((uint32_t)a.pool.vs[at] << 23);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        y0[2 * j] = fp8_pair<0>(y[j], scale), y0[2 * j + 1] = fp8_pair<1>(y[j], scale);
+        y1[2 * j] = fp8_pair<0>(y[2 + j], scale), y1[2 * j + 1] = fp8_pair<1>(y[2 + j], scale);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = __builtin_amdgcn_perm(y1[j / 2], y0[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+      if (eight * 8 + j < rows) *(uint32_t*)(a.v_out + out + (eight * 8 + j) * PAGED_D + d) = eight * 8 + j < len ? w : 0u;
+    }
+  } else if (BITS == 16) {
     u32x4 x0 = {}, x1 = {};
     if (held) {
       const uint16_t* src = (const uint16_t*)(a.pool.k + at * paged_tile_bytes<16>()) + row * PAGED_D + c * 8;
@@ -265,6 +379,7 @@ extern "C" int pbs_paged_append(const void* q, const void* k, const void* v, con
   PBS_REQUIRE(a.q_groups + 2 * Hkv <= 65535, "pbs_paged_append: too many heads");
   const dim3 grid(tiles, a.q_groups + 2 * Hkv, B);
   if (kv_bits == 16) hipLaunchKernelGGL(append_kernel<16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (kv_bits == 8) hipLaunchKernelGGL(append_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(append_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a);
   return pbs_check_launch("pbs_paged_append");
 }
@@ -282,6 +397,7 @@ extern "C" int pbs_paged_read(const void* k_pages, const void* v_pages, const vo
   a.lens = lens; a.k_out = (uint16_t*)k_out; a.v_out = (uint16_t*)v_out; a.L = max_len;
   const dim3 grid((max_len + PAGED_TILE - 1) / PAGED_TILE, Hkv, B);
   if (kv_bits == 16) hipLaunchKernelGGL(read_kernel<16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (kv_bits == 8) hipLaunchKernelGGL(read_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(read_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a);
   return pbs_check_launch("pbs_paged_read");
 }

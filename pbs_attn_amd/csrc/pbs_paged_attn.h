@@ -7,7 +7,6 @@
 #include <math.h>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 constexpr int PAGED_WAVES = 4;       // of a workgroup
 constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequences, at most: two a compute unit
@@ -61,6 +60,11 @@ struct Tile<16> {
   u32x4 k[8], v[8];
 };
 template <>
+struct Tile<8> {
+  u32x4 k[4], v[4];
+  uint32_t ks, vs;
+};
+template <>
 struct Tile<4> {
   u32x4 k[2], v[2];
   uint32_t ks;
@@ -77,6 +81,20 @@ __device__ __forceinline__ void load_v(Tile<16>& t, const PagedPool& p, int64_t 
   const char* v = p.v + at * paged_tile_bytes<16>() + g * 2048 + n * 16;
 #pragma unroll
   for (int d = 0; d < 8; ++d) t.v[d] = *(const u32x4*)(v + d * 256);
+}
+__device__ __forceinline__ void load_k(Tile<8>& t, const PagedPool& p, int64_t at, int n, int g) {
+  const char* k = p.k + at * paged_tile_bytes<8>() + n * 256 + g * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) t.k[h * 2 + c] = *(const u32x4*)(k + h * 128 + c * 64);
+  t.ks = p.ks[at];
+}
+__device__ __forceinline__ void load_v(Tile<8>& t, const PagedPool& p, int64_t at, int n, int g) {   // eight tokens of channels 32 c + 2 n and the next
+  const char* v = p.v + at * paged_tile_bytes<8>() + g * 1024 + n * 16;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) t.v[c] = *(const u32x4*)(v + c * 256);
+  t.vs = p.vs[at];
 }
 __device__ __forceinline__ void load_k(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
   const char* k = p.k + at * paged_tile_bytes<4>() + n * 128 + g * 16;
@@ -114,7 +132,6 @@ struct PagedLater {
     return (up[channel] < seen ? INFINITY : 0.f) - (down[channel] < seen ? INFINITY : 0.f);
   }
 };
-__device__ __forceinline__ bool not_finite(uint32_t bf16_bits) { return (bf16_bits & 0x7f80u) == 0x7f80u; }
 
 // 16 query rows as the matrix instruction's right operand
 template <int BITS>
@@ -143,7 +160,7 @@ struct Rows<16> {
     }
   }
 };
-// For 4-bit keys the queries are the sum of two e4m3 numbers a channel: the matrix instruction then takes the keys as they lie in memory, with
+// For 8- and 4-bit keys the queries are the sum of two e4m3 numbers a channel: the matrix instruction then takes the keys as they lie in memory, with
 // their scales.  A bf16 value has 8 bits, e4m3 4: q = 2^e (hi + lo / 32) with hi = e4m3(q / 2^e) and lo the 4 bits that are left, exact down to 2^-21
 // of the row's largest channel (below it both halves are subnormal and lo is rounded).
 template <>
@@ -203,6 +220,9 @@ struct Rows<4> {
   }
 };
 
+template <>
+struct Rows<8> : Rows<4> {};
+
 // S^T of one half (16 keys, operand row m = token 2 m + half) and 16 query rows
 __device__ __forceinline__ f32x4 logits(const Tile<16>& t, int half, const Rows<16>& r) {
   f32x4 s = {};
@@ -216,6 +236,13 @@ __device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
   f32x4 s = {};
   s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo());
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 4, 0, HALF, (int)t.ks, 0, r.scale_hi);
+}
+__device__ __forceinline__ f32x4 logits(const Tile<8>& t, int half, const Rows<8>& r) {
+  const u32x4 a = t.k[half * 2], b = t.k[half * 2 + 1];
+  const i32x8 k = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+  f32x4 s = {};
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 0, 0, 0, (int)t.ks, 0, r.scale_lo());
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 0, 0, 0, (int)t.ks, 0, r.scale_hi);
 }
 __device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
 

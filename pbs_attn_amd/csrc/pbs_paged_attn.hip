@@ -21,7 +21,7 @@ namespace {
 
 constexpr int O_PITCH = PAGED_D + 4;
 
-// V^T operands: d's holds eight tokens (8 g ..) of channel 16 d + n, of 4-bit pages of channel 8 n + d; here d = 2 c and 2 c + 1.  `held` of the
+// V^T operands: d's holds eight tokens (8 g ..) of channel 16 d + n, of 8-bit pages of channel 32 (d / 2) + 2 n + d % 2, of 4-bit pages of channel 8 n + d; here d = 2 c and 2 c + 1.  `held` of the
 // eight are there.
 template <bool TAIL>
 __device__ __forceinline__ void values(const Tile<16>& t, int c, int held, bf16x8 (&v)[2]) {
@@ -34,6 +34,20 @@ __device__ __forceinline__ void values(const Tile<16>& t, int c, int held, bf16x
     }
     v[e] = __builtin_bit_cast(bf16x8, x);
   }
+}
+template <bool TAIL>
+__device__ __forceinline__ void values(const Tile<8>& t, int c, int held, bf16x8 (&v)[2]) {
+  u32x4 x = t.v[c];
+  float scale = __uint_as_float(t.vs << 23);
+  if (TAIL) {   // (a tile without tokens has no scale either)
+    const uint64_t there = held >= 8 ? ~0ull : held <= 0 ? 0ull : ~0ull >> (64 - 8 * held);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x[w] &= (uint32_t)(there >> (32 * (w & 1)));
+    scale = held > 0 ? scale : 1.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    v[e] = __builtin_bit_cast(bf16x8, (u32x4){fp8_pair<0>(x[2 * e], scale), fp8_pair<1>(x[2 * e], scale), fp8_pair<0>(x[2 * e + 1], scale), fp8_pair<1>(x[2 * e + 1], scale)});
 }
 template <int C>
 __device__ __forceinline__ uint32_t value_pair(uint32_t codes, uint32_t e) {   // channels 2 C and 2 C + 1 of a word
@@ -73,6 +87,19 @@ __device__ __forceinline__ void set_aside(Tile<16>& t, PagedLater& later, int ke
     t.v[d] = x;
   }
 }
+__device__ __forceinline__ void set_aside(Tile<8>& t, PagedLater& later, int key, int held, int n) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    u32x4 x = t.v[c];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (!fp8_is_nan(x[j >> 2] >> (8 * (j & 3)))) continue;
+      if ((j & 7) < held) later.note(c * 32 + n * 2 + (j >> 3), key + (j & 7), 0x7fffu);
+      x[j >> 2] &= ~(0xffu << (8 * (j & 3)));
+    }
+    t.v[c] = x;
+  }
+}
 __device__ __forceinline__ void set_aside(Tile<4>& t, PagedLater& later, int key, int held, int n) {   // (a token's group is NaN or finite)
   u32x2 x = t.vs;
 #pragma unroll
@@ -85,7 +112,7 @@ __device__ __forceinline__ void set_aside(Tile<4>& t, PagedLater& later, int key
   t.vs = x;
 }
 template <int BITS>
-__device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? d * 16 + row : row * 8 + d; }
+__device__ __forceinline__ int channel_of(int d, int row) { return BITS == 16 ? d * 16 + row : BITS == 8 ? (d >> 1) * 32 + row * 2 + (d & 1) : row * 8 + d; }
 
 // One wave's running softmax over its tiles.  S^T = K Q^T leaves a lane with the logits of tokens 8 g .. 8 g + 7 for query row n, which are
 // its share of P^T in O^T += V^T P^T: probabilities never change lanes.
@@ -415,7 +442,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
 
 // Steps of a row tile of `rows`
 constexpr bool through_lds(int rows, int kv_bits) { return rows > (kv_bits == 16 ? 32 : 64); }
-constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : kv_bits == 4 && rows <= 48 ? 256 : 128; }
+constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : (kv_bits == 4 && rows <= 48) || (kv_bits == 8 && rows <= 16) ? 256 : 128; }
 
 struct Plan {
   int rows;      // of a row tile
@@ -426,13 +453,13 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
   max_len = std::min(max_len, PAGED_MAX_TOKENS);
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits == 4 ? 48 : rows <= 64 ? 64 : 128;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits != 16 ? 48 : rows <= 64 ? 64 : 128;
   // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512
   // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.  Many sequences of 700 tokens in
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
   // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  const bool cut = max_len > (kv_bits == 16 ? 640 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
+  const bool cut = max_len > (kv_bits == 16 ? 640 : kv_bits == 8 ? 960 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // (no more workers than there is work for)
   const int64_t steps = units * ((max_len + step_of(p.rows, kv_bits) - 1) / step_of(p.rows, kv_bits));
   p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS, steps + 7) / 8 * 8 : 0;
@@ -492,6 +519,11 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   } else if (kv_bits == 16) {
     if (p.rows == 16) launch<16, 1, 1, 1>(a, st);
     else launch<16, 2, 1, 1>(a, st);
+  } else if (kv_bits == 8) {
+    if (p.rows == 16) launch<8, 1, 2, 1>(a, st);
+    else if (p.rows == 32) launch<8, 2, 1, 1>(a, st);
+    else if (p.rows == 48) launch<8, 3, 1, 1>(a, st);
+    else launch<8, 4, 1, 1>(a, st);
   } else {
     if (p.rows == 16) launch<4, 1, 2, 2>(a, st);
     else if (p.rows == 32) launch<4, 2, 2, 1>(a, st);

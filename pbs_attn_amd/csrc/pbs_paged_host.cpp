@@ -47,23 +47,29 @@ bool rows(const at::Tensor& t) {
 struct Pages {
   at::Tensor k, v, k_scale, v_scale;   // held: another thread may change the pages object while the GIL is released
   int64_t n, heads, size;
+  int bits;
   bool read(PyObject* pk, PyObject* pv, PyObject* pks, PyObject* pvs) {
     const bool bf16 = pks == Py_None && pvs == Py_None;
-    const at::ScalarType type = bf16 ? at::kBFloat16 : at::kByte;
-    const at::Tensor *tk = tensor(pk, type, 4), *tv = tensor(pv, type, bf16 ? 5 : 6);
+    at::ScalarType type = bf16 ? at::kBFloat16 : at::kByte;
+    const at::Tensor* tk = tensor(pk, type, 4);
+    const bool fp8 = !bf16 && !tk;
+    if (fp8) tk = tensor(pk, type = at::kFloat8_e4m3fn, 4);
+    const at::Tensor* tv = tensor(pv, type, bf16 || fp8 ? 5 : 6);
     if (!tk || !tv) return false;
     k = *tk, v = *tv;
+    bits = bf16 ? 16 : fp8 ? 8 : 4;
     if (!bf16) {
-      const at::Tensor *tks = tensor(pks, type, 5), *tvs = tensor(pvs, type, 5);
+      const at::Tensor *tks = tensor(pks, at::kByte, fp8 ? 3 : 5), *tvs = tensor(pvs, at::kByte, fp8 ? 3 : 5);
       if (!tks || !tvs) return false;
       k_scale = *tks, v_scale = *tvs;
     }
     n = k.size(0), heads = k.size(1), size = k.size(2);
     if (n <= 0 || heads <= 0 || (size != 32 && size != 64 && size != 128 && size != 256)) return false;
-    if (bf16 ? !is_shape(k, {n, heads, size, HEAD_DIM}) || !is_shape(v, {n, heads, size / 8, HEAD_DIM, 8})
+    if (bits != 4 ? !is_shape(k, {n, heads, size, HEAD_DIM}) || !is_shape(v, {n, heads, size / 8, HEAD_DIM, 8})
              : !is_shape(k, {n, heads, size, HEAD_DIM / 2}) || !is_shape(v, {n, heads, size / 4, 16, 4, 4}) ||
                    !is_shape(k_scale, {n, heads, size / 32, 4, 32}) || !is_shape(v_scale, {n, heads, size / 32, 4, 32}))
       return false;
+    if (fp8 && (!is_shape(k_scale, {n, heads, size / 32}) || !is_shape(v_scale, {n, heads, size / 32}))) return false;
     for (const at::Tensor* t : {&k, &v, &k_scale, &v_scale})
       if (t->defined() && (!t->is_contiguous() || !aligned(t->const_data_ptr()) || t->device() != k.device())) return false;
     return true;
@@ -79,7 +85,6 @@ struct Pages {
   const void* vp() const { return v.const_data_ptr(); }
   const void* ksp() const { return k_scale.defined() ? k_scale.const_data_ptr() : nullptr; }
   const void* vsp() const { return v_scale.defined() ? v_scale.const_data_ptr() : nullptr; }
-  int bits() const { return k_scale.defined() ? 4 : 16; }
 };
 
 const at::Tensor* table_of(PyObject* x, int64_t B) {
@@ -163,7 +168,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   rc = append_fn(address(q), address(k), address(v), address(cos), address(sin), q ? q_out.mutable_data_ptr() : nullptr,
                  k_out.defined() ? k_out.mutable_data_ptr() : nullptr, kp, vp, ksp, vsp,
                  (const int32_t*)address(table), (const int32_t*)address(past), (const int32_t*)address(fresh), (int)B, (int)Hq, (int)Hkv, (int)S, HEAD_DIM,
-                 (int)pages.n, (int)table->size(1), (int)pages.size, pages.bits(), q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? q->stride(2) : 0,
+                 (int)pages.n, (int)table->size(1), (int)pages.size, pages.bits, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? q->stride(2) : 0,
                  k->stride(0), k->stride(1), k->stride(2), v->stride(0), v->stride(1), v->stride(2), cos && cos->size(0) > 1 ? cos->stride(0) : 0,
                  cos ? cos->stride(1) : 0, table->stride(0), stream);
   Py_END_ALLOW_THREADS
@@ -200,14 +205,14 @@ PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (max_len <= 0) return not_taken();
   void* stream;
   if (!stream_of(*q, &stream)) return not_taken();
-  const size_t bytes = attn_bytes_fn((int)B, (int)Hq, (int)pages.heads, (int)S, HEAD_DIM, pages.bits(), (int)max_len);
+  const size_t bytes = attn_bytes_fn((int)B, (int)Hq, (int)pages.heads, (int)S, HEAD_DIM, pages.bits, (int)max_len);
   at::Tensor out = at::empty({B, Hq, S, HEAD_DIM}, q->options()), ws;
   if (bytes) ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = attn_fn(q->const_data_ptr(), pages.kp(), pages.vp(), pages.ksp(), pages.vsp(), (const int32_t*)table->const_data_ptr(),
                (const int32_t*)past->const_data_ptr(), fresh ? (const int32_t*)fresh->const_data_ptr() : nullptr, out.mutable_data_ptr(), (int)B, (int)Hq,
-               (int)pages.heads, (int)S, HEAD_DIM, (int)pages.n, (int)table->size(1), (int)pages.size, pages.bits(), (int)max_len, q->stride(0),
+               (int)pages.heads, (int)S, HEAD_DIM, (int)pages.n, (int)table->size(1), (int)pages.size, pages.bits, (int)max_len, q->stride(0),
                q->stride(1), q->stride(2), Hq * S * HEAD_DIM, S * HEAD_DIM, HEAD_DIM, table->stride(0), scale,
                bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream);
   Py_END_ALLOW_THREADS
@@ -234,7 +239,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_BEGIN_ALLOW_THREADS
   rc = read_fn(pages.kp(), pages.vp(), pages.ksp(), pages.vsp(), (const int32_t*)table->const_data_ptr(), (const int32_t*)lens->const_data_ptr(),
                k.mutable_data_ptr(), v.mutable_data_ptr(), (int)B, (int)pages.heads, (int)L, HEAD_DIM, (int)pages.n, (int)table->size(1), (int)pages.size,
-               pages.bits(), table->stride(0), stream);
+               pages.bits, table->stride(0), stream);
   Py_END_ALLOW_THREADS
   if (rc) return failed(rc, "pbs_paged_read");
   PyObject *a = THPVariable_Wrap(std::move(k)), *b = THPVariable_Wrap(std::move(v));

@@ -409,7 +409,7 @@ def _check_paged(pages, page_table, B, Hkv, lens, *ts):
     for t in (*ts, page_table, *lens):
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {t.device} and pages on {device}")
-    return n, page_table.shape[1], page_size, 16 if pages.k_scale is None else 4
+    return n, page_table.shape[1], page_size, pages.bits
 
 
 def _on_device_of(t):
@@ -427,7 +427,8 @@ def paged_append(pages, page_table, past_lens, k, v, q=None, cos=None, sin=None,
     with one rounding at the end; without them nothing is rotated.  All tensors on one GPU, lengths and table int32.
     Returns (q, k) rotated, contiguous and head-major, all S rows: q (B, Hq, S, 128) where one is given, k with ``want_k``, else None.
 
-    Tokens whose page is not in the pool or that lie behind the table are not stored.  At most one sequence may write to a page."""
+    Tokens whose page is not in the pool or that lie behind the table are not stored.  At most one sequence may write to a page.  In 8 bits
+    the tokens of a block of 32 (positions 32 t .. 32 t + 31) that are there already are rounded again where new ones take its scale up."""
     done = (_lib._paged_host or _lib.paged_host()).append(pages, page_table, past_lens, k, v, q, cos, sin, new_lens, want_k)
     if done is not None:
         return done

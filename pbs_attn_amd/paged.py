@@ -1,5 +1,5 @@
 """A paged key-value cache: the pages of a layer (``KVPages``, ``alloc_pages``), which ``ops.paged_append`` writes, ``ops.paged_attn``
-attends to and ``ops.paged_read`` reads back, in bf16 or in 4 bits."""
+attends to and ``ops.paged_read`` reads back, in bf16, 8 or 4 bits."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -11,7 +11,8 @@ from . import _lib
 
 PAGE_SIZES = (32, 64, 128, 256)
 HEAD_DIM = 128
-FORMATS = ("bf16", "fp4")
+FORMATS = ("bf16", "fp4", "fp8")
+FP8 = torch.float8_e4m3fn
 
 
 @dataclass
@@ -19,6 +20,9 @@ class KVPages:
     """One layer's pages of P tokens, head-major.
 
     bf16: ``k`` (pages, heads, P, 128), ``v`` (pages, heads, P / 8, 128, 8) with the eight tokens of a channel side by side.
+
+    8 bits (``k`` and ``v`` float8_e4m3fn): their layouts as in bf16, and a power of two for 32 tokens of a head, as its exponent + 127:
+    ``k_scale``, ``v_scale`` (pages, heads, P / 32) uint8.
 
     4 bits (``k_scale`` and ``v_scale`` given): uint8, two e2m1 codes a byte, the even channel in the low half: ``k`` (pages, heads, P, 64),
     ``v`` (pages, heads, P / 4, 16, 4, 4) = (token / 4, channel / 8, token % 4, byte), and a power of two for 32 channels of a token, as its
@@ -42,20 +46,29 @@ class KVPages:
         if ks is None and vs is None:
             ok = k.dtype == v.dtype == torch.bfloat16 and last == HEAD_DIM and v.shape == (n, h, p // 8, HEAD_DIM, 8)
             tensors = (k, v)
+        elif k.dtype == FP8:
+            ok = (ks is not None and vs is not None and v.dtype == FP8 and ks.dtype == vs.dtype == torch.uint8 and last == HEAD_DIM
+                  and v.shape == (n, h, p // 8, HEAD_DIM, 8) and ks.shape == vs.shape == (n, h, p // 32))
+            tensors = (k, v, ks, vs)
         else:
             ok = (ks is not None and vs is not None and k.dtype == v.dtype == ks.dtype == vs.dtype == torch.uint8 and last == HEAD_DIM // 2
                   and v.shape == (n, h, p // 4, 16, 4, 4) and ks.shape == vs.shape == (n, h, p // 32, 4, 32))
             tensors = (k, v, ks, vs)
         if not ok or n == 0 or h == 0:
             raise ValueError("pages are either bf16 K (pages, heads, P, 128) and V (pages, heads, P / 8, 128, 8), or uint8 K (.., P, 64) and "
-                             "V (.., P / 4, 16, 4, 4) with two scales (.., P / 32, 4, 32)")
+                             "V (.., P / 4, 16, 4, 4) with two scales (.., P / 32, 4, 32), or float8_e4m3fn in the shapes of bf16 with two uint8 "
+                             "scales (.., P / 32)")
         for t in tensors:
             if not t.is_contiguous() or t.device != k.device or t.data_ptr() % 16:
                 raise ValueError("the pages of a layer are contiguous, 16-byte aligned tensors on one device")
 
     @property
     def form(self) -> str:
-        return "bf16" if self.k_scale is None else "fp4"
+        return "bf16" if self.k_scale is None else "fp8" if self.k.dtype == FP8 else "fp4"
+
+    @property
+    def bits(self) -> int:
+        return {"bf16": 16, "fp8": 8, "fp4": 4}[self.form]
 
     @property
     def page_size(self) -> int:
@@ -76,4 +89,6 @@ def alloc_pages(num_pages, num_kv_heads, page_size=64, form="bf16", device="cuda
         return torch.empty(shape, dtype=dtype, device=device)
     if form == "bf16":
         return KVPages(empty(n, h, p, HEAD_DIM, dtype=torch.bfloat16), empty(n, h, p // 8, HEAD_DIM, 8, dtype=torch.bfloat16))
+    if form == "fp8":
+        return KVPages(empty(n, h, p, HEAD_DIM, dtype=FP8), empty(n, h, p // 8, HEAD_DIM, 8, dtype=FP8), empty(n, h, p // 32), empty(n, h, p // 32))
     return KVPages(empty(n, h, p, HEAD_DIM // 2), empty(n, h, p // 4, 16, 4, 4), empty(n, h, p // 32, 4, 32), empty(n, h, p // 32, 4, 32))

@@ -123,8 +123,9 @@ class _PagedLayer(CacheLayerMixin):
 
 
 class PagedKVCache(Cache):
-    """Room for ``batch_size`` sequences of up to ``max_len`` tokens of a model with ``config``, in pages of ``page_size`` tokens, bf16 or
-    4 bits (``form="fp4"``: about a quarter of the memory and of a decoding step's traffic; the first prompt's own attention still sees bf16).
+    """Room for ``batch_size`` sequences of up to ``max_len`` tokens of a model with ``config``, in pages of ``page_size`` tokens, bf16,
+    8 bits (``form="fp8"``: half of the memory and of a decoding step's traffic) or 4 bits (``form="fp4"``: about a quarter); the first prompt's own
+    attention still sees bf16.
     ``num_kv_heads``: of this process, where it is not the configuration's (tensor parallel)."""
 
     is_paged = True

@@ -237,12 +237,14 @@ __device__ __forceinline__ f32x4 logits4(const Tile<4>& t, const Rows<4>& r) {
   s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 4, 0, HALF, (int)t.ks, 0, r.scale_lo());
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 4, 0, HALF, (int)t.ks, 0, r.scale_hi);
 }
+__device__ __forceinline__ f32x4 logits8(const i32x8& k, uint32_t scale, const Rows<8>& r) {
+  f32x4 s = {};
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 0, 0, 0, (int)scale, 0, r.scale_lo());
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 0, 0, 0, (int)scale, 0, r.scale_hi);
+}
 __device__ __forceinline__ f32x4 logits(const Tile<8>& t, int half, const Rows<8>& r) {
   const u32x4 a = t.k[half * 2], b = t.k[half * 2 + 1];
-  const i32x8 k = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-  f32x4 s = {};
-  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.lo, s, 0, 0, 0, (int)t.ks, 0, r.scale_lo());
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, r.hi, s, 0, 0, 0, (int)t.ks, 0, r.scale_hi);
+  return logits8((i32x8){(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]}, t.ks, r);
 }
 __device__ __forceinline__ f32x4 logits(const Tile<4>& t, int half, const Rows<4>& r) { return half ? logits4<1>(t, r) : logits4<0>(t, r); }
 
@@ -384,5 +386,19 @@ __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& 
   if (threadIdx.x == 0) a.headers[worker] = {s.b * a.row_tiles + at.tile, at.head, more, 0};
 }
 
-// many rows a row tile (csrc/pbs_paged_rows.hip)
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+  return ((uint64_t)hi << 32) | (uint64_t)lo;
+}
+
+// 1 KB from `base` + each lane's offset to LDS byte `to` + 16 a lane, without waiting (vmcnt).  (The s_nop: wait states between the scalar
+// registers' writes and the copy.)
+__device__ __forceinline__ void copy_async(uint64_t base, uint32_t offset, uint32_t to) {
+  register uint32_t m0v asm("m0") = to;
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(offset), "s"(base) : "memory");
+}
+
+// many rows a row tile (csrc/pbs_paged_rows.hip; 8 bits: csrc/pbs_paged_rows8.hip)
 int paged_attn_rows(const PagedAttnArgs& a, int kv_bits, int rows, hipStream_t stream);
+int paged_attn_rows8(const PagedAttnArgs& a, hipStream_t stream);

@@ -1,8 +1,8 @@
 // Attention over a paged cache for prompts behind a filled cache and drafted tokens: 64 or 128 query rows a workgroup.
 //
 // The mathematics and the row numbering are those of pbs_paged_attn.hip.  Here the waves share the keys and split the rows (16 or 32 each), so
-// tiles of 64 keys go through LDS, two buffers: bf16 tiles are copied there asynchronously; values in 8 and 4 bits are loaded into registers during
-// the tile before and unpacked to bf16 behind it, once for all rows, while keys in 8 and 4 bits need no unpacking and go to every wave's registers
+// tiles of 64 keys go through LDS, two buffers: bf16 tiles are copied there asynchronously; values in 4 bits are loaded into registers during
+// the tile before and unpacked to bf16 behind it, once for all rows, while keys in 4 bits need no unpacking and go to every wave's registers
 // as they are.
 //
 // A wave's order within a step keeps both units busy: the logits of its second 32 keys beside the weights of the first, the products of the
@@ -30,19 +30,6 @@ extern __shared__ __attribute__((aligned(16))) char lds[];
 // bf16 K: rows of 256 bytes, the 16-byte chunk j of row r in place j ^ (r / 2 % 16): an operand's sixteen lanes read rows 2 n + half.
 __device__ __forceinline__ int k_place(int row, int chunk) { return row * 256 + ((chunk ^ ((row >> 1) & 15)) * 16); }
 
-__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
-  return ((uint64_t)hi << 32) | (uint64_t)lo;
-}
-
-// 1 KB from `base` + each lane's offset to LDS byte `to` + 16 a lane, without waiting (vmcnt).  (The s_nop: wait states between the scalar
-// registers' writes and the copy.)
-__device__ __forceinline__ void copy_async(uint64_t base, uint32_t offset, uint32_t to) {
-  register uint32_t m0v asm("m0") = to;
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(offset), "s"(base) : "memory");
-}
-
 // The next tile of 64 keys on its way into LDS.  A half of 32 keys whose page is not there is read as the pool's first tile, and masked.
 template <int BITS>
 struct Stage;
@@ -66,35 +53,6 @@ struct Stage<16> {
     for (int i = 0; i < 4; ++i) copy_async(v, (uint32_t)(lane * 16 + i * 1024), buffer + (uint32_t)(lds_v(16) + wave * 4096 + i * 1024));
   }
   __device__ __forceinline__ void store(uint32_t buffer, int held0, int held1) {}   // (the copies are awaited by all waves before the barrier)
-};
-template <>
-struct Stage<8> {
-  u32x4 v[2];       // eight tokens of two channels, of either half
-  uint32_t vs[2];
-  __device__ __forceinline__ void begin(int, int) {}
-  __device__ __forceinline__ void load(const PagedPool& p, int64_t at0, int64_t at1, uint32_t, int, int) {
-    v[0] = *(const u32x4*)(p.v + at0 * paged_tile_bytes<8>() + threadIdx.x * 16);
-    v[1] = *(const u32x4*)(p.v + at1 * paged_tile_bytes<8>() + threadIdx.x * 16);
-    vs[0] = p.vs[at0];
-    vs[1] = p.vs[at1];
-  }
-  // `held`: tokens of either half that are there; the others' codes may be NaN, and the scale of a half without tokens too
-  __device__ __forceinline__ void store(uint32_t buffer, int held0, int held1) {
-    const int m = threadIdx.x & 63, eight = threadIdx.x >> 6;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int held = (half ? held1 : held0) - eight * 8;
-      const uint64_t there = held >= 8 ? ~0ull : held <= 0 ? 0ull : ~0ull >> (64 - 8 * held);
-      const float scale = held > 0 ? __uint_as_float(vs[half] << 23) : 1.f;
-      // place 64 e + m holds channel 2 m + e
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t lo = v[half][2 * e] & (uint32_t)there, hi = v[half][2 * e + 1] & (uint32_t)(there >> 32);
-        *(u32x4*)(lds + buffer + lds_v(8) + ((half * 4 + eight) * PAGED_D + e * 64 + m) * 16) =
-            (u32x4){fp8_pair<0>(lo, scale), fp8_pair<1>(lo, scale), fp8_pair<0>(hi, scale), fp8_pair<1>(hi, scale)};
-      }
-    }
-  }
 };
 template <>
 struct Stage<4> {
@@ -137,10 +95,6 @@ struct Stage<4> {
     }
   }
 };
-
-// the channel whose values lie in place `at` of a group of eight tokens
-template <int BITS>
-__device__ __forceinline__ int channel_at(int at) { return BITS == 16 ? at : BITS == 8 ? (at & 63) * 2 + (at >> 6) : (at & 15) * 8 + (at >> 4); }
 
 template <int BITS, int RW>   // RW: 16-row tiles of a wave
 __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u, int head, int s0, int steps, float* part) {
@@ -185,11 +139,11 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   int64_t at0, at1;
   int held0 = 0, held1 = 0, next0 = 0, next1 = 0;
   uint32_t buffer = 0;
-  Tile<BITS == 16 ? 4 : BITS> keys[2];   // (8 and 4 bits)
+  Tile<4> keys[2];   // (4 bits)
   if (s0 < end) {
     look_up(s0, at0, at1, held0, held1);
     stage.load(a.pool, at0, at1, buffer, wave, lane);
-    if (BITS != 16) {
+    if (BITS == 4) {
       load_k(keys[0], a.pool, at0, n, g);
       load_k(keys[1], a.pool, at1, n, g);
     }
@@ -228,7 +182,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
         for (int j = 0; j < 8; ++j) {
           const uint32_t h = x[j >> 1] >> (16 * (j & 1)) & 0xffffu;
           if (!not_finite(h)) continue;
-          later.note(channel_at<BITS>(place), key + j, h);
+          later.note(BITS == 16 ? place : (place & 15) * 8 + (place >> 4), key + j, h);
           x[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
         }
         *at = x;
@@ -325,7 +279,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       }
     }
     fence();
-    if (BITS != 16 && step + 1 < end) {
+    if (BITS == 4 && step + 1 < end) {
       load_k(keys[0], a.pool, at0, n, g);
       load_k(keys[1], a.pool, at1, n, g);
     }
@@ -364,14 +318,14 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[r][d][i] += later.of(channel_at<BITS>(d * 16 + 4 * g + i), u.past + token + 1);
+        for (int i = 0; i < 4; ++i) o[r][d][i] += later.of(BITS == 16 ? d * 16 + 4 * g + i : (4 * g + i) * 8 + d, u.past + token + 1);
     }
     if (part) {
       if (token >= u.fresh) continue;   // (cleared by the join)
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[rr * PAGED_D + channel_at<BITS>(d * 16 + 4 * g + i)] = o[r][d][i];
+        for (int i = 0; i < 4; ++i) part[rr * PAGED_D + (BITS == 16 ? d * 16 + 4 * g + i : (4 * g + i) * 8 + d)] = o[r][d][i];
       if (g == 0) *(f32x2*)(part + ROWS * PAGED_D + rr * 2) = (f32x2){m[r], sum};
     } else if (token < a.S) {
       const float scale = sum == 0.f || token >= u.fresh ? 0.f : 1.f / sum;   // (rows without a token weigh the keys that every row sees)
@@ -382,10 +336,6 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       if (BITS == 16) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) *(u32x2*)(dst + d * 16 + 4 * g) = (u32x2){two(o[r][d][0], o[r][d][1]), two(o[r][d][2], o[r][d][3])};
-      } else if (BITS == 8) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-          *(u32x4*)(dst + d * 32 + 8 * g) = (u32x4){two(o[r][d][0], o[r][d + 4][0]), two(o[r][d][1], o[r][d + 4][1]), two(o[r][d][2], o[r][d + 4][2]), two(o[r][d][3], o[r][d + 4][3])};
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -422,5 +372,5 @@ int launch(const PagedAttnArgs& a, hipStream_t stream) {
 
 int paged_attn_rows(const PagedAttnArgs& a, int kv_bits, int rows, hipStream_t stream) {
   if (kv_bits == 16) return rows == 64 ? launch<16, 1>(a, stream) : launch<16, 2>(a, stream);
-  return kv_bits == 8 ? launch<8, 2>(a, stream) : launch<4, 2>(a, stream);
+  return kv_bits == 8 ? paged_attn_rows8(a, stream) : launch<4, 2>(a, stream);
 }

@@ -18,7 +18,7 @@ constexpr int PAGED_WORKERS = 512;   // workgroups of a launch that cuts sequenc
 constexpr float PAGED_SLACK = 8.f;
 
 struct PagedHeader {   // of a worker: the piece of work that it began and left to the `more` workers after it
-  int unit, head, more, pad;
+  int unit, head, more, fresh;   // fresh: the sequence's new tokens (the join has no other reason to look at the lengths)
 };
 
 struct PagedAttnArgs {
@@ -52,6 +52,83 @@ __device__ __forceinline__ int paged_lane() {
   return l;
 }
 
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+  return ((uint64_t)hi << 32) | (uint64_t)lo;
+}
+
+// A pool of 8 bits as one sequence and head see it, held in registers.  (Left to the compiler the pool's description is read from the kernel's
+// arguments again in every step, one round trip to the scalar cache after the other: 900 cycles of the 3700 that a wave's step of 64 keys and 32
+// rows took.)
+struct HeadPool {
+  uint64_t k, v, ks, vs, row;   // the head's first tile of page 0, and the sequence's row of the table
+  uint32_t page_tiles;          // tiles from a page to the next
+  int tiles_shift, num_pages, last_slot;
+  __device__ __forceinline__ HeadPool(const PagedPool& p, int b, int head) {
+    tiles_shift = p.page_shift - 5, num_pages = p.num_pages, last_slot = p.max_pages - 1;
+    page_tiles = (uint32_t)p.heads << tiles_shift;
+    const uint64_t first = (uint64_t)head << tiles_shift;
+    k = uniform64((uint64_t)p.k + first * paged_tile_bytes<8>());
+    v = uniform64((uint64_t)p.v + first * paged_tile_bytes<8>());
+    ks = uniform64((uint64_t)p.ks + first);
+    vs = uniform64((uint64_t)p.vs + first);
+    row = uniform64((uint64_t)(p.table + b * p.table_sb));
+    asm volatile("" : "+s"(k), "+s"(v), "+s"(ks), "+s"(vs), "+s"(row), "+s"(page_tiles), "+s"(tiles_shift), "+s"(num_pages), "+s"(last_slot));
+  }
+};
+
+// Where a wave's tiles lie: `NT` of them from `first` on in each of its steps, `stride` tiles from one step to the next.
+//
+// 16 and 4 bits: the page table is read in front of a step's loads.  8 bits: a lane holds the pages of one of the next 64 steps.
+template <int BITS, int NT>
+struct Places {
+  const PagedPool& p;
+  const int b, head, first, stride, tiles;
+  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int first, int stride, int tiles)
+      : p(a.pool), b(b), head(head), first(first), stride(stride), tiles(tiles) {}
+  __device__ __forceinline__ const PagedPool& pool() const { return p; }
+  // of step `i` (counted from `first`): bit j of the result: tile j is not there, and its place is that of the pool's first tile
+  __device__ __forceinline__ uint32_t look_up(int i, int64_t (&at)[NT]) {
+    uint32_t none = 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int t = first + i * stride + j;
+      at[j] = t < tiles ? paged_tile_index(p, b, head, t) : -1;
+      none |= (at[j] < 0 ? 1u : 0u) << j;
+      at[j] = max(at[j], (int64_t)0);
+    }
+    return none;
+  }
+};
+template <int NT>
+struct Places<8, NT> {
+  const HeadPool p;
+  const int first, stride, tiles;
+  int page[NT];
+  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int first, int stride, int tiles)
+      : p(a.pool, b, head), first(first), stride(stride), tiles(tiles) {}
+  __device__ __forceinline__ const HeadPool& pool() const { return p; }
+  __device__ __forceinline__ uint32_t look_up(int i, int64_t (&at)[NT]) {
+    if ((i & 63) == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int t = first + (i + (int)(threadIdx.x & 63)) * stride + j;
+        page[j] = t >= 0 && t < tiles ? ((const int32_t*)p.row)[min(t >> p.tiles_shift, p.last_slot)] : -1;   // (keys end with the table)
+      }
+    }
+    uint32_t none = 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int x = __builtin_amdgcn_readlane(page[j], i & 63);
+      const bool there = (unsigned)x < (unsigned)p.num_pages;
+      none |= (there ? 0u : 1u) << j;
+      at[j] = (int64_t)((uint64_t)(uint32_t)(there ? x : 0) * p.page_tiles + ((first + i * stride + j) & ((1 << p.tiles_shift) - 1)));
+    }
+    return none;
+  }
+};
+
 // What a lane holds of a tile of 32 tokens.  n = lane % 16, g = lane / 16.
 template <int BITS>
 struct Tile;
@@ -82,19 +159,21 @@ __device__ __forceinline__ void load_v(Tile<16>& t, const PagedPool& p, int64_t 
 #pragma unroll
   for (int d = 0; d < 8; ++d) t.v[d] = *(const u32x4*)(v + d * 256);
 }
-__device__ __forceinline__ void load_k(Tile<8>& t, const PagedPool& p, int64_t at, int n, int g) {
-  const char* k = p.k + at * paged_tile_bytes<8>() + n * 256 + g * 16;
+__device__ __forceinline__ void load_k(Tile<8>& t, const HeadPool& p, int64_t at, int n, int g) {
+  const char* k = (const char*)(p.k + at * paged_tile_bytes<8>());
+  const uint32_t from = n * 256 + g * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) t.k[h * 2 + c] = *(const u32x4*)(k + h * 128 + c * 64);
-  t.ks = p.ks[at];
+    for (int c = 0; c < 2; ++c) t.k[h * 2 + c] = *(const u32x4*)(k + (from + h * 128 + c * 64));
+  t.ks = ((const uint8_t*)p.ks)[at];
 }
-__device__ __forceinline__ void load_v(Tile<8>& t, const PagedPool& p, int64_t at, int n, int g) {   // eight tokens of channels 32 c + 2 n and the next
-  const char* v = p.v + at * paged_tile_bytes<8>() + g * 1024 + n * 16;
+__device__ __forceinline__ void load_v(Tile<8>& t, const HeadPool& p, int64_t at, int n, int g) {   // eight tokens of channels 32 c + 2 n and the next
+  const char* v = (const char*)(p.v + at * paged_tile_bytes<8>());
+  const uint32_t from = g * 1024 + n * 16;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) t.v[c] = *(const u32x4*)(v + c * 256);
-  t.vs = p.vs[at];
+  for (int c = 0; c < 4; ++c) t.v[c] = *(const u32x4*)(v + (from + c * 256));
+  t.vs = ((const uint8_t*)p.vs)[at];
 }
 __device__ __forceinline__ void load_k(Tile<4>& t, const PagedPool& p, int64_t at, int n, int g) {
   const char* k = p.k + at * paged_tile_bytes<4>() + n * 128 + g * 16;
@@ -288,15 +367,15 @@ struct PagedShare {
   int b, head, tile, step, todo, share;
 };
 struct PagedShareLds {
-  int wave_sums[PAGED_WAVES], left, b;
+  int wave_sums[2 * PAGED_WAVES], left, b;
 };
-template <int ROWS, int STEP>
+template <int ROWS, int STEP, int WAVES>
 __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int workers, PagedShare* out) {
   int total = 0, before = 0, mine = 0, from = 0;
   if (a.B == 1) {
     total = a.Hkv * paged_seq<ROWS, STEP>(a, 0).a_head;
   } else {   // running sums over the sequences, a stretch of them a thread
-    const int tid = threadIdx.x, stretch = (a.B + 255) / 256, to = min((tid + 1) * stretch, a.B);
+    const int tid = threadIdx.x, stretch = (a.B + WAVES * 64 - 1) / (WAVES * 64), to = min((tid + 1) * stretch, a.B);
     from = min(tid * stretch, a.B);
     for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
     before = mine;
@@ -309,7 +388,7 @@ __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLd
     before -= mine;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < PAGED_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       if (w < (tid >> 6)) before += lds.wave_sums[w];
       total += lds.wave_sums[w];
     }
@@ -350,11 +429,11 @@ __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLd
 
 // A workgroup's way through its share, or through the one row tile and head that are its without headers: work(unit, head, first step,
 // steps, part), part null where the steps are all that the row tile has.
-template <int ROWS, int STEP, class Work>
+template <int ROWS, int STEP, int WAVES, class Work>
 __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& lds, int worker, bool last_tile_first, Work&& work) {
   PagedShare at;
   if (a.headers) {
-    if (!paged_share<ROWS, STEP>(a, lds, worker, gridDim.x, &at)) {
+    if (!paged_share<ROWS, STEP, WAVES>(a, lds, worker, gridDim.x, &at)) {
       if (threadIdx.x == 0) a.headers[worker].more = 0;
       return;
     }
@@ -383,13 +462,7 @@ __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& 
       }
     }
   }
-  if (threadIdx.x == 0) a.headers[worker] = {s.b * a.row_tiles + at.tile, at.head, more, 0};
-}
-
-__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
-  return ((uint64_t)hi << 32) | (uint64_t)lo;
+  if (threadIdx.x == 0) a.headers[worker] = {s.b * a.row_tiles + at.tile, at.head, more, s.fresh};
 }
 
 // 1 KB from `base` + each lane's offset to LDS byte `to` + 16 a lane, without waiting (vmcnt).  (The s_nop: wait states between the scalar

@@ -123,7 +123,10 @@ struct Softmax {
   RowsLds* lds;
   f32x4 o[R][8];
   float m[R];
-  f32x4 l[R];   // the weights' sums, as products with ones (every row of the tile the same): 32 bits, on the matrix unit, and no sum over lanes
+  // The weights' sums, in 32 bits: as products with ones on the matrix unit (every row of the tile the same, and no sum over lanes), 8 bits of the lane's
+  // own tokens by the vector unit, two at a time (three registers a row tile less: with them the loads go out a step earlier).
+  static constexpr bool LANE_SUMS = BITS == 8;
+  typename std::conditional<LANE_SUMS, float, f32x4>::type l[R];
   int seen[R];
 
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedUnit& u, int head, int n, int g, int wave, RowsLds* q_lds) {
@@ -138,7 +141,7 @@ struct Softmax {
       }
       seen[r] = valid ? u.past + token + 1 : 0;
       m[r] = -FLT_MAX;
-      l[r] = (f32x4){};
+      l[r] = {};
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[r][d] = (f32x4){};
     }
@@ -197,8 +200,27 @@ struct Softmax {
         // bf16, as the matrix instruction takes them: half a step is 2^-8 of a weight, above the line and below it
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[r][i][j] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i][j], c, -m[r]));
-        l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i], l[r], 0, 0, 0);
+        if constexpr (LANE_SUMS) {
+          const u32x4 w = __builtin_bit_cast(u32x4, p[r][i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t two = w[j];
+            l[r] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), (bf16x2){(__bf16)1.f, (__bf16)1.f}, l[r], false);
+          }
+        } else {
+          l[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][i], l[r], 0, 0, 0);
+        }
       }
+  }
+  __device__ __forceinline__ float sum(int r) const {
+    if constexpr (LANE_SUMS) {
+      TwoOf t = with_lane_xor<16>(__float_as_uint(l[r]));
+      const float two = __uint_as_float(t.a) + __uint_as_float(t.b);
+      t = with_lane_xor<32>(__float_as_uint(two));
+      return __uint_as_float(t.a) + __uint_as_float(t.b);
+    } else {
+      return l[r][0];
+    }
   }
   template <bool TAIL>
   __device__ __forceinline__ void add(const Tile<BITS> (&t)[NT], const bf16x8 (&p)[R][NT], int k0, int keys, uint32_t gone, int g) {
@@ -237,39 +259,37 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   Tile<BITS> tile[DEPTH][NT];
   uint32_t gone[DEPTH] = {};
   int64_t at[NT];
-  auto look_up = [&](int t) __attribute__((always_inline)) {
-    uint32_t none = 0;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      at[i] = t + i < tiles ? paged_tile_index(a.pool, u.b, head, t + i) : -1;
-      none |= (at[i] < 0 ? 1u : 0u) << i;
-      at[i] = max(at[i], (int64_t)0);
-    }
-    return none;
-  };
+  int step = 0;
+  Places<BITS, NT> places(a, u.b, head, t, STRIDE, tiles);
   if (t < end) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (t + d * STRIDE >= end) break;
-      gone[d] = look_up(t + d * STRIDE);
+      gone[d] = places.look_up(d, at);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) load_k(tile[d][i], a.pool, at[i], n, g);
+      for (int i = 0; i < NT; ++i) load_k(tile[d][i], places.pool(), at[i], n, g);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) load_v(tile[d][i], a.pool, at[i], n, g);
+      for (int i = 0; i < NT; ++i) load_v(tile[d][i], places.pool(), at[i], n, g);
     }
   }
   auto one = [&](auto mask, Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
     const int next = t + DEPTH * STRIDE, k0 = t * PAGED_TILE;
+    // (the older waves of a compute unit would finish a third earlier and leave the memory half idle: they go first in every other step only.
+    // 8 bits: 128k tokens of one sequence 58.6 -> 57.3 us, 128 sequences 374 -> 365)
+    if (BITS == 8 && R == 1) {
+      if ((blockIdx.x >= gridDim.x / 2) == (step & 1)) __builtin_amdgcn_s_setprio(0);
+      else __builtin_amdgcn_s_setprio(2);
+    }
     // (with several row tiles the loads behind the last step repeat its own: without the branches 35 rows take 68 us for 73; with one row
     // tile the steps are short, and the wait for what nobody uses costs 2 %)
     const bool load = R > 1 || next < end;
     uint32_t gone_next = 0;
-    if (load) gone_next = look_up(R == 1 || next < end ? next : t);
+    if (load) gone_next = places.look_up(R == 1 || next < end ? step + DEPTH : step, at);
     bf16x8 p[R][NT];
     s.template weigh<mask.value>(tile, p, k0, u.keys, gone, a.scale_log2, a.room, n, g);
     if (load) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) load_k(tile[i], a.pool, at[i], n, g);
+      for (int i = 0; i < NT; ++i) load_k(tile[i], places.pool(), at[i], n, g);
     }
     if (mask.value && mixed && k0 + NT * PAGED_TILE > u.all_see) {
 #pragma unroll
@@ -282,10 +302,11 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     s.template add<mask.value>(tile, p, k0, u.keys, gone, g);
     if (load) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) load_v(tile[i], a.pool, at[i], n, g);
+      for (int i = 0; i < NT; ++i) load_v(tile[i], places.pool(), at[i], n, g);
     }
     gone = gone_next;
     t += STRIDE;
+    ++step;
   };
   // (tiles that every row sees whole, then the rest: those at the end, and whatever follows a page that is not there)
   const int seen_whole = min(u.all_see, u.keys) / PAGED_TILE - NT;
@@ -318,7 +339,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   bool noted = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float l = s.l[r][0];
+    const float l = s.sum(r);
     if (r > 0) __syncthreads();   // (the rows before have been read)
     if (g2 == 0) {
       ml_lds[wave][n2][0] = s.m[r];
@@ -329,10 +350,19 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, ml_lds[w][n2][0]);
     const float f = __builtin_amdgcn_exp2f(s.m[r] - top);
+    if constexpr (BITS == 8) {   // (a lane's channels lie in eights)
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
+      for (int d = 0; d < 8; d += 2)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = s.o[r][d][i] * f;
+        for (int i = 0; i < 4; i += 2)
+          *(f32x4*)&o_lds[wave][n2][channel_of<8>(d, 4 * g2 + i)] =
+              (f32x4){s.o[r][d][i] * f, s.o[r][d + 1][i] * f, s.o[r][d][i + 1] * f, s.o[r][d + 1][i + 1] * f};
+    } else {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o_lds[wave][n2][channel_of<BITS>(d, 4 * g2 + i)] = s.o[r][d][i] * f;
+    }
     __syncthreads();
     if (r == 0) noted = mixed && later.is_any();
     // 16 lanes a row, 8 channels a lane
@@ -374,12 +404,12 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
 
 template <int BITS, int R, int NT, int DEPTH, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_kernel(PagedAttnArgs a) {
-  __shared__ float o_lds[WAVES][16][O_PITCH];
+  __shared__ __attribute__((aligned(16))) float o_lds[WAVES][16][O_PITCH];
   __shared__ float ml_lds[WAVES][16][2];
   __shared__ PagedShareLds share_lds;
   __shared__ RowsLds q_lds[R > 1 ? R : 1];
   __shared__ PagedLater later;
-  paged_go<R * 16, WAVES * NT * PAGED_TILE>(a, share_lds, blockIdx.x, false, [&](const PagedUnit& u, int head, int step, int steps, float* part)
+  paged_go<R * 16, WAVES * NT * PAGED_TILE, WAVES>(a, share_lds, blockIdx.x, false, [&](const PagedUnit& u, int head, int step, int steps, float* part)
                                             __attribute__((always_inline)) { work<BITS, R, NT, DEPTH, WAVES>(a, u, head, step, steps, part, o_lds, ml_lds, q_lds, later); });
 }
 
@@ -390,7 +420,7 @@ template <int GROUPS>
 __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
   const PagedHeader h = a.headers[blockIdx.x];
   if (h.more == 0) return;
-  const int b = h.unit / a.row_tiles, fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
+  const int b = h.unit / a.row_tiles, fresh = h.fresh;
   const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, share = group % GROUPS;
   const int rr = blockIdx.y * (16 / GROUPS) + group / GROUPS, row = (h.unit - b * a.row_tiles) * rows + rr, token = row / a.G;
   if (GROUPS == 16 && token >= a.S) return;
@@ -399,17 +429,29 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
   float top = -FLT_MAX, sum = 0.f;
   f32x4 y0 = {}, y1 = {};
   if (token < fresh) {
-#pragma unroll 4
-    for (int i = share; i <= h.more; i += GROUPS) {
-      // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
-      const float* p = first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot);
-      const f32x2 ml = *(const f32x2*)(p + rows * PAGED_D + rr * 2);
-      const f32x4 x0 = *(const f32x4*)(p + rr * PAGED_D + lane * 8), x1 = *(const f32x4*)(p + rr * PAGED_D + lane * 8 + 4);
-      const float m = fmaxf(top, ml.x), old = __builtin_amdgcn_exp2f(top - m), now = __builtin_amdgcn_exp2f(ml.x - m);
-      top = m;
-      sum = sum * old + ml.y * now;
-      y0 = y0 * old + x0 * now;
-      y1 = y1 * old + x1 * now;
+    // (four parts at a time, all of their loads before the first is used: one after the other, behind a look at the count each, they took
+    // the join of 64 parts a row 3 us longer)
+    for (int i0 = share; i0 <= h.more; i0 += 4 * GROUPS) {
+      f32x2 ml[4];
+      f32x4 x0[4], x1[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = min(i0 + j * GROUPS, h.more);
+        // part i > 0: slot 0 of worker blockIdx.x + i, one slot and i - 1 pairs of slots further on
+        const float* p = first + (i == 0 ? 0 : (int64_t)(2 * i - 1) * slot);
+        ml[j] = *(const f32x2*)(p + rows * PAGED_D + rr * 2);
+        x0[j] = *(const f32x4*)(p + rr * PAGED_D + lane * 8), x1[j] = *(const f32x4*)(p + rr * PAGED_D + lane * 8 + 4);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i0 + j * GROUPS > h.more) break;
+        const float m = fmaxf(top, ml[j].x), old = __builtin_amdgcn_exp2f(top - m), now = __builtin_amdgcn_exp2f(ml[j].x - m);
+        top = m;
+        sum = sum * old + ml[j].y * now;
+        y0 = y0 * old + x0[j] * now;
+        y1 = y1 * old + x1[j] * now;
+      }
     }
   }
   if (GROUPS > 1) {
@@ -440,13 +482,15 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
       (u32x4){two(y0[0], y0[1]), two(y0[2], y0[3]), two(y1[0], y1[1]), two(y1[2], y1[3])};
 }
 
-// Steps of a row tile of `rows`
+// Keys of a step of a row tile of `rows`, where a workgroup has four waves
 constexpr bool through_lds(int rows, int kv_bits) { return rows > (kv_bits == 16 ? 32 : 64); }
 constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits) ? 64 : (kv_bits == 4 && rows <= 48) || (kv_bits == 8 && rows <= 16) ? 256 : 128; }
 
 struct Plan {
   int rows;      // of a row tile
   int workers;   // 0: sequences are not cut
+  int waves;     // of a worker
+  int step;      // its keys
   size_t bytes;
 };
 Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
@@ -459,18 +503,30 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
   // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  const bool cut = max_len > (kv_bits == 16 ? 640 : kv_bits == 8 ? 960 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
+  // 8 bits, uncut against cut: one sequence of 700 tokens 8.8 us against 9.8, 1003 10.2 against 10.2, 1300 11.9 against 10.1; where whole units fill half
+  // the chip, up to a workgroup a compute unit, longer ones too: 16 of 2000 16.2 against 18.9, of 3000 25.0 against 23.7, 32 of 3000 38.4 against
+  // 42.2; 8 of 1300 12.8 against 13.8, of 3000 20.1 against 18.1; five tokens of each, 4 KV heads, 8 of 2000 23.9 against 25.9, 64 of 1003 20.5 against 26.5.
+  const int64_t row_tiles = units * p.rows / 16;
+  const int least8 = units > 256 || row_tiles < 48 ? 1000 : row_tiles < 96 ? 1600 : 2700;
+  const bool cut = max_len > (kv_bits == 16 ? 640 : kv_bits == 8 ? least8 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
+  // One worker of eight waves a compute unit instead of two of four: half as many parts, and no older workgroup that goes ahead.  8 bits, with one row
+  // tile and few, long units: 128k tokens of one sequence 58.6 -> 55.9 us, 4 KV heads 39.1 -> 35.8, 32 sequences of 8000 tokens 56.3 -> 54.6.  Not
+  // where a worker's share is a step or two (one sequence of 4100 tokens 11.1 -> 11.8, of 16000 15.2 -> 16.0), nor where it crosses from unit to
+  // unit, as nothing runs beside the end of one (64 sequences of 17 .. 8191 tokens, 4 KV heads 62.2 -> 68.8).
+  p.waves = 4, p.step = step_of(p.rows, kv_bits);
+  if (kv_bits == 8 && p.rows == 16 && units <= 128 && units * ((max_len + 511) / 512) >= PAGED_WORKERS) p.waves = 8, p.step = 512;
   // (no more workers than there is work for)
-  const int64_t steps = units * ((max_len + step_of(p.rows, kv_bits) - 1) / step_of(p.rows, kv_bits));
-  p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS, steps + 7) / 8 * 8 : 0;
+  const int64_t steps = units * ((max_len + p.step - 1) / p.step);
+  p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS * 4 / p.waves, steps + 7) / 8 * 8 : 0;
   p.bytes = p.workers * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows));
   return p;
 }
 
-// NT tiles a wave and step, DEPTH steps ahead.  Without cuts a workgroup has eight waves, and several row tiles leave each half the registers.
+// NT tiles a wave and step, DEPTH steps ahead.  `waves`: of a worker.  Without cuts a workgroup has eight waves, and several row tiles leave each half the registers.
 template <int BITS, int R, int NT, int DEPTH>
-void launch(const PagedAttnArgs& a, hipStream_t stream) {
-  if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), dim3(a.workers), dim3(256), 0, stream, a);
+void launch(const PagedAttnArgs& a, hipStream_t stream, int waves = 4) {
+  if (a.headers && BITS == 8 && R == 1 && waves == 8) hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), dim3(a.workers), dim3(512), 0, stream, a);
+  else if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), dim3(a.workers), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), dim3(a.Hkv * a.B * a.row_tiles), dim3(512), 0, stream, a);
 }
 
@@ -509,7 +565,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   const int64_t units = (int64_t)B * Hkv * a.row_tiles;
   PBS_REQUIRE(units < (1 << 22), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
   // the line of steps that workers share has to fit 32 bits, whatever the lengths turn out to be: a call that may not is not cut
-  if (units * ((int64_t)max_pages * page_size / step_of(p.rows, kv_bits) + 1) > INT32_MAX) p.workers = 0;
+  if (units * ((int64_t)max_pages * page_size / p.step + 1) > INT32_MAX) p.workers = 0;
   a.workers = p.workers;
   a.headers = p.workers ? (PagedHeader*)workspace : nullptr;
   a.parts = p.workers ? (float*)((char*)workspace + p.workers * sizeof(PagedHeader)) : nullptr;
@@ -520,7 +576,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
     if (p.rows == 16) launch<16, 1, 1, 1>(a, st);
     else launch<16, 2, 1, 1>(a, st);
   } else if (kv_bits == 8) {
-    if (p.rows == 16) launch<8, 1, 2, 1>(a, st);
+    if (p.rows == 16) launch<8, 1, 2, 1>(a, st, p.waves);
     else if (p.rows == 32) launch<8, 2, 1, 1>(a, st);
     else if (p.rows == 48) launch<8, 3, 1, 1>(a, st);
     else launch<8, 4, 1, 1>(a, st);

@@ -31,25 +31,6 @@ __device__ __forceinline__ int k_place(int pair, int chunk) { return pair * 256 
 // V: 16 bytes are eight tokens of a channel; place 64 e + m of a group of eight holds channel 2 m + e
 __device__ __forceinline__ int channel_at(int place) { return (place & 63) * 2 + (place >> 6); }
 
-// The pool as one sequence and head see it, held in registers.  (Left to the compiler they are read from the kernel's arguments again in every
-// step, one round trip to the scalar cache after the other: 900 cycles of a wave's 3700.)
-struct HeadPool {
-  uint64_t k, v, ks, vs, row;   // the head's first tile of page 0, and the sequence's row of the table
-  uint32_t page_tiles;          // tiles from a page to the next
-  int tiles_shift, num_pages, last_slot;
-  __device__ __forceinline__ HeadPool(const PagedPool& p, int b, int head) {
-    tiles_shift = p.page_shift - 5, num_pages = p.num_pages, last_slot = p.max_pages - 1;
-    page_tiles = (uint32_t)p.heads << tiles_shift;
-    const uint64_t first = (uint64_t)head << tiles_shift;
-    k = uniform64((uint64_t)p.k + first * paged_tile_bytes<8>());
-    v = uniform64((uint64_t)p.v + first * paged_tile_bytes<8>());
-    ks = uniform64((uint64_t)p.ks + first);
-    vs = uniform64((uint64_t)p.vs + first);
-    row = uniform64((uint64_t)(p.table + b * p.table_sb));
-    asm volatile("" : "+s"(k), "+s"(v), "+s"(ks), "+s"(vs), "+s"(row), "+s"(page_tiles), "+s"(tiles_shift), "+s"(num_pages), "+s"(last_slot));
-  }
-};
-
 // the tile of 64 keys after the one at hand.  A half of 32 keys whose page is not there is read as the pool's first tile of the head, and
 // masked.  The page table is read a step ahead; steps behind the last load what is not used.
 struct Next {
@@ -298,11 +279,13 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       hide(step, 1);
       const int v_next = v_at == LDS_V + 2 * V_BYTES ? LDS_V : v_at + V_BYTES;
       fence();
+      __builtin_amdgcn_s_setprio(1);
       next.store(lds + v_next);
       add();
       const bool grows = look(1);
       beside_products<5>();
       fence();
+      __builtin_amdgcn_s_setprio(0);
       grow(grows);
       read_v(1);     // (the last of this tile)
       k_at ^= K_BYTES;
@@ -318,11 +301,13 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       fence();
       hide(step, 0);
       fence();
+      __builtin_amdgcn_s_setprio(1);
       read_k(1);
       add();
       const bool grows_next = look(0);
       beside_products<1>();
       fence();
+      __builtin_amdgcn_s_setprio(0);
       grow(grows_next);
     }
     read_v(0);
@@ -375,7 +360,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows8_kernel(PagedAttnArgs a) {
   // Workers that follow each other read the same head's keys at the same time: they go to one of the eight dies and its L2 (workgroups
   // are dealt to them in turn).  Without cuts the heads follow each other, and the row tiles that see the most keys come first.
   const int worker = a.headers ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : 0;
-  paged_go<ROWS, KEYS>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true, [&](const PagedUnit& u, int head, int step, int steps, float* part)
+  paged_go<ROWS, KEYS, WAVES>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true, [&](const PagedUnit& u, int head, int step, int steps, float* part)
                        __attribute__((always_inline)) { work(a, u, head, step, steps, part); });
 }
 

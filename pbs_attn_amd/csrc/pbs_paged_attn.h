@@ -334,7 +334,7 @@ struct PagedSeq {
   int a_head;        // steps of one head: row tiles without tokens take one, in which their rows are cleared
   int tiles;         // row tiles with tokens
 };
-template <int ROWS, int STEP>
+template <int ROWS, int STEP, int EXTRA>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b) {
   PagedSeq s;
   s.b = b;
@@ -342,7 +342,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int b) {
   s.fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;
   s.tiles = (s.fresh * a.G + ROWS - 1) / ROWS;
   s.steps = max((min(s.past + s.fresh, a.pool.max_pages << a.pool.page_shift) + STEP - 1) / STEP, 1);
-  s.a_head = s.tiles * s.steps + (a.row_tiles - s.tiles);
+  s.a_head = s.tiles * (s.steps + EXTRA) + (a.row_tiles - s.tiles);
   return s;
 }
 struct PagedUnit {
@@ -363,21 +363,22 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedAttnArgs& a, int b, i
 
 // Where a workgroup begins, and how many steps are its.  The steps of all sequences lie in one line (sequence, head, row tile, step), cut
 // into equal shares, one a worker, so that sequences of any lengths fill the chip.  (The host sees to it that the line's length fits 32 bits.)
+// A row tile of a head stands in the line with EXTRA steps in front of its own: what a worker takes to begin a piece, and to end the one before.
 struct PagedShare {
   int b, head, tile, step, todo, share;
 };
 struct PagedShareLds {
   int wave_sums[2 * PAGED_WAVES], left, b;
 };
-template <int ROWS, int STEP, int WAVES>
+template <int ROWS, int STEP, int EXTRA, int WAVES>
 __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLds& lds, int worker, int workers, PagedShare* out) {
   int total = 0, before = 0, mine = 0, from = 0;
   if (a.B == 1) {
-    total = a.Hkv * paged_seq<ROWS, STEP>(a, 0).a_head;
+    total = a.Hkv * paged_seq<ROWS, STEP, EXTRA>(a, 0).a_head;
   } else {   // running sums over the sequences, a stretch of them a thread
     const int tid = threadIdx.x, stretch = (a.B + WAVES * 64 - 1) / (WAVES * 64), to = min((tid + 1) * stretch, a.B);
     from = min(tid * stretch, a.B);
-    for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+    for (int i = from; i < to; ++i) mine += a.Hkv * paged_seq<ROWS, STEP, EXTRA>(a, i).a_head;
     before = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -404,7 +405,7 @@ __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLd
     if (start >= before && start < before + mine) {
       left = start - before;
       for (int i = from;; ++i) {
-        const int cost = a.Hkv * paged_seq<ROWS, STEP>(a, i).a_head;
+        const int cost = a.Hkv * paged_seq<ROWS, STEP, EXTRA>(a, i).a_head;
         if (left < cost) {
           lds.b = i;
           lds.left = left;
@@ -417,23 +418,25 @@ __device__ __forceinline__ bool paged_share(const PagedAttnArgs& a, PagedShareLd
     b = __builtin_amdgcn_readfirstlane(lds.b);
     left = __builtin_amdgcn_readfirstlane(lds.left);
   }
-  const PagedSeq s = paged_seq<ROWS, STEP>(a, b);
-  const int full = s.tiles * s.steps;
+  const PagedSeq s = paged_seq<ROWS, STEP, EXTRA>(a, b);
+  const int in_line = s.steps + EXTRA, full = s.tiles * in_line;
   out->b = b;
   out->head = left / s.a_head;
   left -= out->head * s.a_head;
-  out->tile = left < full ? left / s.steps : s.tiles + (left - full);
-  out->step = left < full ? left - out->tile * s.steps : 0;
-  return true;
+  out->tile = left < full ? left / in_line : s.tiles + (left - full);
+  const int at = left < full ? left - out->tile * in_line : EXTRA;
+  out->step = max(at - EXTRA, 0);
+  out->todo -= max(EXTRA - at, 0);
+  return out->todo > 0;   // (not where the share ends before the first step)
 }
 
 // A workgroup's way through its share, or through the one row tile and head that are its without headers: work(unit, head, first step,
 // steps, part), part null where the steps are all that the row tile has.
-template <int ROWS, int STEP, int WAVES, class Work>
+template <int ROWS, int STEP, int EXTRA, int WAVES, class Work>
 __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& lds, int worker, bool last_tile_first, Work&& work) {
   PagedShare at;
   if (a.headers) {
-    if (!paged_share<ROWS, STEP, WAVES>(a, lds, worker, gridDim.x, &at)) {
+    if (!paged_share<ROWS, STEP, EXTRA, WAVES>(a, lds, worker, gridDim.x, &at)) {
       if (threadIdx.x == 0) a.headers[worker].more = 0;
       return;
     }
@@ -443,7 +446,7 @@ __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& 
     at.share = at.todo = INT32_MAX;
   }
   int more = 0;
-  PagedSeq s = paged_seq<ROWS, STEP>(a, at.b);
+  PagedSeq s = paged_seq<ROWS, STEP, EXTRA>(a, at.b);
   while (true) {
     const int steps = at.tile < s.tiles ? s.steps : 1, n = min(steps - at.step, at.todo);
     at.todo -= n;
@@ -458,8 +461,12 @@ __device__ __forceinline__ void paged_go(const PagedAttnArgs& a, PagedShareLds& 
       at.tile = 0;
       if (++at.head == a.Hkv) {
         at.head = 0;
-        s = paged_seq<ROWS, STEP>(a, s.b + 1);
+        s = paged_seq<ROWS, STEP, EXTRA>(a, s.b + 1);
       }
+    }
+    if (EXTRA > 0 && at.tile < s.tiles) {
+      if (at.todo <= EXTRA) break;   // (the next worker begins it)
+      at.todo -= EXTRA;
     }
   }
   if (threadIdx.x == 0) a.headers[worker] = {s.b * a.row_tiles + at.tile, at.head, more, s.fresh};

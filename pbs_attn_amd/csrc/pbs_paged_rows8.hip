@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows8_kernel(PagedAttnArgs a) {
   // Workers that follow each other read the same head's keys at the same time: they go to one of the eight dies and its L2 (workgroups
   // are dealt to them in turn).  Without cuts the heads follow each other, and the row tiles that see the most keys come first.
   const int worker = a.headers ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : 0;
-  paged_go<ROWS, KEYS, WAVES>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true, [&](const PagedUnit& u, int head, int step, int steps, float* part)
+  paged_go<ROWS, KEYS, 0, WAVES>(a, *(PagedShareLds*)(lds + LDS_SHARE), worker, true, [&](const PagedUnit& u, int head, int step, int steps, float* part)
                        __attribute__((always_inline)) { work(a, u, head, step, steps, part); });
 }
 

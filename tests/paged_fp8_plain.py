@@ -98,3 +98,20 @@ def check_untouched(before, after, touched):
                 for kv in range(2):
                     (_, a, e), (_, b, f) = block_of(before, page, t, kv), block_of(after, page, t, kv)
                     assert torch.equal(a, b) and torch.equal(e, f), (page, t, kv)
+
+
+def held_after(pieces):
+    """What a cache that is empty holds of tokens that come in pieces (heads, n, 128): (heads, all, 128) float64."""
+    out, e_now = torch.zeros(pieces[0].shape[0], 0, 128, dtype=torch.float64, device=pieces[0].device), None
+    for x in pieces:
+        x = x.double()
+        while x.shape[1]:
+            at = out.shape[1] % BLOCK
+            new, x = x[:, :BLOCK - at], x[:, BLOCK - at:]
+            e = exponent_of(new)
+            if at:
+                e = torch.maximum(e, e_now)
+            unit, before = two_to(e)[:, None, None], out.shape[1] - at
+            out = torch.cat((out[:, :before], rounded(out[:, before:] / unit) * unit, rounded(new / unit) * unit), 1)
+            e_now = e
+    return out

@@ -2,7 +2,7 @@
 //
 // The mathematics and the row numbering are those of pbs_paged_attn.hip.  As in pbs_paged_rows.hip the waves share the keys and split the rows,
 // 32 each, and tiles of 64 keys go through LDS: keys as they are, by asynchronous copies (8 KB, two buffers), values unpacked to bf16 on the
-// way, once for all rows (16 KB, three buffers).
+// way, once for all rows (16 KB, two buffers).
 //
 // A step has 512 cycles of the matrix unit for its logits (the queries are two e4m3 numbers a channel), 576 for its products, and about 1000 of
 // the vector unit, half of them exponentials.  So the order is one where each stretch of matrix instructions has vector work beside it that
@@ -21,7 +21,7 @@ constexpr int WAVES = PAGED_WAVES, RW = 2;   // RW: 16-row tiles of a wave
 constexpr int ROWS = WAVES * RW * 16;
 constexpr int KEYS = 64;                     // of a step
 constexpr int K_BYTES = KEYS * PAGED_D, V_BYTES = KEYS * PAGED_D * 2;
-constexpr int LDS_V = 2 * K_BYTES, LDS_LATER = LDS_V + 3 * V_BYTES, LDS_SHARE = LDS_LATER + (int)sizeof(PagedLater);
+constexpr int LDS_V = 2 * K_BYTES, LDS_LATER = LDS_V + 2 * V_BYTES, LDS_SHARE = LDS_LATER + (int)sizeof(PagedLater);
 constexpr int LDS_TOTAL = LDS_SHARE + (int)sizeof(PagedShareLds);
 
 extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -277,7 +277,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       fence();
       next.hide(wave);
       hide(step, 1);
-      const int v_next = v_at == LDS_V + 2 * V_BYTES ? LDS_V : v_at + V_BYTES;
+      const int v_next = 2 * LDS_V + V_BYTES - v_at;
       fence();
       __builtin_amdgcn_s_setprio(1);
       next.store(lds + v_next);

@@ -432,8 +432,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttnArgs a, int rows) {
   float top = -FLT_MAX, sum = 0.f;
   f32x4 y0 = {}, y1 = {};
   if (token < fresh) {
-    // (four parts at a time, all of their loads before the first is used: one after the other, behind a look at the count each, they took
-    // the join of 64 parts a row 3 us longer)
+    // (four parts at a time, all of their loads before the first is used: with 64 parts a row 0.4 us less than a look at the count before each)
     for (int i0 = share; i0 <= h.more; i0 += 4 * GROUPS) {
       f32x2 ml[4];
       f32x4 x0[4], x1[4];

@@ -4,13 +4,14 @@
 // j <= past + i, m the largest exponent so far (one pass: sums are rescaled where it grows).  All query heads of a KV head and several
 // tokens share a tile's rows, row r = (token r / G, head r % G of the group), so a key is read once for all of them.
 //
-// Here: up to 32 rows of a bf16 cache, up to 64 of a 4-bit one; pbs_paged_rows.hip takes more.  Bound by memory, so the waves of a workgroup split
+// Here: up to 32 rows of a bf16 cache, up to 64 of an 8- or 4-bit one; pbs_paged_rows.hip and pbs_paged_rows8.hip take more.  Bound by memory, so the waves of a workgroup split
 // the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order and nothing is shared
 // but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
 // parts), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
 // 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their
 // time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 13 registers of a wave
-// go to scratch memory, 20 with eight waves.)
+// go to scratch memory, 20 with eight waves.)  In 8 bits 128k tokens take 57 us (5.2 TB/s in this launch, then a join of 5 us; reading as much and
+// nothing else 44.5), 128 sequences 366 (5.8), 35 rows of 16 sequences 64 (4.4).
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>

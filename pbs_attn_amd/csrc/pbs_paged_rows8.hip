@@ -12,6 +12,11 @@
 //    (barrier: the next tile is in LDS)
 //    logits of the next's first half    beside   weights of the second half
 //    products of the second half        beside   maxima of the next's first half
+//
+// 1000 new tokens behind 32k (32 / 8 heads) 487 us, 1.12 PFLOP/s (with the logits' two parts counted, 1.68), 500 of two sequences behind up to 16k 212.  By the
+// counters the matrix unit works 51 % of the time and the vector unit 50 %, at 2.25 GHz: an 8-bit matrix instruction keeps the vector unit's issue for
+// about 20 cycles and a bf16 one for 8, so what does run beside them is less than it looks.  With instructions of 32 rows the cycles are 3 % fewer
+// and the clock 6 % lower (2.11 GHz): 533 us for 514 at that time.
 #include "pbs_paged_attn.h"
 #include <math.h>
 
@@ -92,6 +97,7 @@ struct Next {
 
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 // The order within a stretch: after each matrix instruction some of the vector unit's (2), of its exponentials (0x400) and reads from LDS (0x100).
+// (Left to the compiler the matrix instructions end up behind the vector work: 501 us for 493; five vector instructions behind a product 493, three 489.)
 __device__ __forceinline__ void beside_logits() {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -279,11 +285,11 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
       hide(step, 1);
       const int v_next = 2 * LDS_V + V_BYTES - v_at;
       fence();
-      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_s_setprio(1);   // (the wave that multiplies values goes before the one that weighs: 517 -> 501 us)
       next.store(lds + v_next);
       add();
       const bool grows = look(1);
-      beside_products<5>();
+      beside_products<3>();
       fence();
       __builtin_amdgcn_s_setprio(0);
       grow(grows);

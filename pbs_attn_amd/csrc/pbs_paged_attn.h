@@ -78,23 +78,21 @@ struct HeadPool {
   }
 };
 
-// Where a wave's tiles lie: `NT` of them from `first` on in each of its steps, `stride` tiles from one step to the next.
+// Where a wave's tiles lie: `NT` of them in each of its steps, `stride` tiles from one step to the next.
 //
 // 16 and 4 bits: the page table is read in front of a step's loads.  8 bits: a lane holds the pages of one of the next 64 steps.
 template <int BITS, int NT>
 struct Places {
   const PagedPool& p;
-  const int b, head, first, stride, tiles;
-  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int first, int stride, int tiles)
-      : p(a.pool), b(b), head(head), first(first), stride(stride), tiles(tiles) {}
+  const int b, head, tiles;
+  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int, int tiles) : p(a.pool), b(b), head(head), tiles(tiles) {}
   __device__ __forceinline__ const PagedPool& pool() const { return p; }
-  // of step `i` (counted from `first`): bit j of the result: tile j is not there, and its place is that of the pool's first tile
-  __device__ __forceinline__ uint32_t look_up(int i, int64_t (&at)[NT]) {
+  // of step `i`, whose first tile is `t`: bit j of the result: tile j is not there, and its place is that of the pool's first tile
+  __device__ __forceinline__ uint32_t look_up(int, int t, int64_t (&at)[NT]) {
     uint32_t none = 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int t = first + i * stride + j;
-      at[j] = t < tiles ? paged_tile_index(p, b, head, t) : -1;
+      at[j] = t + j < tiles ? paged_tile_index(p, b, head, t + j) : -1;
       none |= (at[j] < 0 ? 1u : 0u) << j;
       at[j] = max(at[j], (int64_t)0);
     }
@@ -104,17 +102,17 @@ struct Places {
 template <int NT>
 struct Places<8, NT> {
   const HeadPool p;
-  const int first, stride, tiles;
+  const int stride, tiles;
   int page[NT];
-  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int first, int stride, int tiles)
-      : p(a.pool, b, head), first(first), stride(stride), tiles(tiles) {}
+  __device__ __forceinline__ Places(const PagedAttnArgs& a, int b, int head, int stride, int tiles)
+      : p(a.pool, b, head), stride(stride), tiles(tiles) {}
   __device__ __forceinline__ const HeadPool& pool() const { return p; }
-  __device__ __forceinline__ uint32_t look_up(int i, int64_t (&at)[NT]) {
+  __device__ __forceinline__ uint32_t look_up(int i, int first_of, int64_t (&at)[NT]) {
     if ((i & 63) == 0) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int t = first + (i + (int)(threadIdx.x & 63)) * stride + j;
-        page[j] = t >= 0 && t < tiles ? ((const int32_t*)p.row)[min(t >> p.tiles_shift, p.last_slot)] : -1;   // (keys end with the table)
+        const int t = first_of + (int)(threadIdx.x & 63) * stride + j;
+        page[j] = t < tiles ? ((const int32_t*)p.row)[min(t >> p.tiles_shift, p.last_slot)] : -1;   // (keys end with the table)
       }
     }
     uint32_t none = 0;
@@ -123,7 +121,7 @@ struct Places<8, NT> {
       const int x = __builtin_amdgcn_readlane(page[j], i & 63);
       const bool there = (unsigned)x < (unsigned)p.num_pages;
       none |= (there ? 0u : 1u) << j;
-      at[j] = (int64_t)((uint64_t)(uint32_t)(there ? x : 0) * p.page_tiles + ((first + i * stride + j) & ((1 << p.tiles_shift) - 1)));
+      at[j] = (int64_t)((uint64_t)(uint32_t)(there ? x : 0) * p.page_tiles + ((first_of + j) & ((1 << p.tiles_shift) - 1)));
     }
     return none;
   }

@@ -261,12 +261,12 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   uint32_t gone[DEPTH] = {};
   int64_t at[NT];
   int step = 0;
-  Places<BITS, NT> places(a, u.b, head, t, STRIDE, tiles);
+  Places<BITS, NT> places(a, u.b, head, STRIDE, tiles);
   if (t < end) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (t + d * STRIDE >= end) break;
-      gone[d] = places.look_up(d, at);
+      gone[d] = places.look_up(d, t + d * STRIDE, at);
 #pragma unroll
       for (int i = 0; i < NT; ++i) load_k(tile[d][i], places.pool(), at[i], n, g);
 #pragma unroll
@@ -285,7 +285,7 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
     // tile the steps are short, and the wait for what nobody uses costs 2 %)
     const bool load = R > 1 || next < end;
     uint32_t gone_next = 0;
-    if (load) gone_next = places.look_up(R == 1 || next < end ? step + DEPTH : step, at);
+    if (load) gone_next = places.look_up(R == 1 || next < end ? step + DEPTH : step, R == 1 || next < end ? next : t, at);
     bf16x8 p[R][NT];
     s.template weigh<mask.value>(tile, p, k0, u.keys, gone, a.scale_log2, a.room, n, g);
     if (load) {

@@ -50,7 +50,8 @@ __device__ __forceinline__ uint32_t largest_finite_bits(uint32_t x) {
   const uint32_t lo = x & 0x7fffu, hi = (x >> 16) & 0x7fffu;
   return max(not_finite(lo) ? 0u : lo, not_finite(hi) ? 0u : hi);
 }
-// the largest over the workgroup
+// The largest over the workgroup.  (Of exponents, and not of magnitudes: every thread has used what it read of the tile's scale when the first one
+// goes on to write it.)
 __device__ __forceinline__ uint32_t max_of_group(uint32_t m, uint32_t (&lds)[4]) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     for (int j = 0; j < 8; ++j) w[j] = s0 + j >= 0 && s0 + j < fresh ? *(const uint32_t*)(src + (int64_t)(s0 + j) * a.v_ss) : 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, largest_finite_bits(w[j]));
-    const uint32_t e = max(e_old, fp8_scale_byte(max_of_group(m, most)));
+    const uint32_t e = max_of_group(max(e_old, fp8_scale_byte(m)), most);
     const float scale = __uint_as_float(e << 23), was = __uint_as_float(e_old << 23);
 #pragma unroll
     for (int c2 = 0; c2 < 2; ++c2)
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = max(m, max(largest_finite_bits(x0[i]), largest_finite_bits(x1[i])));
       }
-      const uint32_t e = max(e_old, fp8_scale_byte(max_of_group(m, most)));
+      const uint32_t e = max_of_group(max(e_old, fp8_scale_byte(m)), most);
       const float scale = __uint_as_float(e << 23), was = __uint_as_float(e_old << 23);
       if (s < 0) {
 #pragma unroll

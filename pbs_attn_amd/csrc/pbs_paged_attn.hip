@@ -492,7 +492,7 @@ constexpr int step_of(int rows, int kv_bits) { return through_lds(rows, kv_bits)
 struct Plan {
   int rows;      // of a row tile
   int workers;   // 0: sequences are not cut
-  int waves;     // of a worker
+  int waves;     // of a workgroup
   int step;      // its keys
   size_t bytes;
 };
@@ -506,11 +506,12 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
   // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  // 8 bits, uncut against cut: one sequence of 700 tokens 8.8 us against 9.8, 1003 10.2 against 10.2, 1300 11.9 against 10.1; where whole units fill half
-  // the chip, up to a workgroup a compute unit, longer ones too: 16 of 2000 16.2 against 18.9, of 3000 25.0 against 23.7, 32 of 3000 38.4 against
-  // 42.2; 8 of 1300 12.8 against 13.8, of 3000 20.1 against 18.1; five tokens of each, 4 KV heads, 8 of 2000 23.9 against 25.9, 64 of 1003 20.5 against 26.5.
-  const int64_t row_tiles = units * p.rows / 16;
-  const int least8 = units > 256 || row_tiles < 48 ? 1000 : row_tiles < 96 ? 1600 : 2700;
+  // 8 bits, uncut against cut: one sequence of 700 tokens 8.1 us against 10.6, 1003 10.2 against 10.2, 1300 11.9 against 10.1; where whole units fill half
+  // the chip longer ones too: 16 of 2000 16.2 against 18.9, of 3000 25.0 against 23.7, 8 of 1300 12.8 against 13.8, of 3000 20.1 against 18.1; where they
+  // are more than it takes at once and of any lengths: 64 of 10 .. 1000 17.6 against 22.0, .. 2000 33.6 against 35.4, .. 3000 49.0 against 48.3, 64 of
+  // 17 .. 8191, 4 KV heads 64.5 against 60.4; five tokens of 128, 4 KV heads, 10 .. 1000 23.2 against 33.3, of 32, 10 .. 2600 26.1 against 24.8.
+  const int64_t row_tiles = units * p.rows / 16;   // (4 sequences of 1000, 32 units, 10.3 against 12.4)
+  const int least8 = row_tiles < 48 ? 1100 : row_tiles < 96 ? 1600 : units <= 256 && p.rows == 16 ? 2700 : 2000;
   const bool cut = max_len > (kv_bits == 16 ? 640 : kv_bits == 8 ? least8 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // One worker of eight waves a compute unit instead of two of four: half as many parts, and no older workgroup that goes ahead.  8 bits, with one row
   // tile and few, long units: 128k tokens of one sequence 58.6 -> 55.9 us, 4 KV heads 39.1 -> 35.8, 32 sequences of 8000 tokens 56.3 -> 54.6.  Not
@@ -521,16 +522,20 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // (no more workers than there is work for)
   const int64_t steps = units * ((max_len + p.step - 1) / p.step);
   p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS * 4 / p.waves, steps + 7) / 8 * 8 : 0;
+  // Whole units have eight waves each where a compute unit has no second one to run beside it and a few steps to share: 8 bits, 16 sequences of 1500 tokens 13.7 us
+  // against 14.3 with four, five tokens of 32 sequences of 1000, 4 KV heads, 17.7 against 19.4; but one sequence of 27 tokens 6.2 against 5.8, of 500 7.8
+  // against 7.1, 128 of 500 40.0 against 30.0.
+  if (!cut && !through_lds(p.rows, kv_bits)) p.waves = kv_bits == 8 && (units > 256 || max_len <= (p.rows == 16 ? 1000 : 500)) ? 4 : 8;
   p.bytes = p.workers * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows));
   return p;
 }
 
-// NT tiles a wave and step, DEPTH steps ahead.  `waves`: of a worker.  Without cuts a workgroup has eight waves, and several row tiles leave each half the registers.
+// NT tiles a wave and step, DEPTH steps ahead; with eight waves several row tiles leave each half the registers.
 template <int BITS, int R, int NT, int DEPTH>
-void launch(const PagedAttnArgs& a, hipStream_t stream, int waves = 4) {
-  if (a.headers && BITS == 8 && R == 1 && waves == 8) hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), dim3(a.workers), dim3(512), 0, stream, a);
-  else if (a.headers) hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), dim3(a.workers), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), dim3(a.Hkv * a.B * a.row_tiles), dim3(512), 0, stream, a);
+void launch(const PagedAttnArgs& a, int waves, hipStream_t stream) {
+  const dim3 grid(a.headers ? a.workers : a.Hkv * a.B * a.row_tiles);
+  if (waves == 8) hipLaunchKernelGGL((attn_kernel<BITS, R, R == 1 ? NT : 1, R == 1 ? DEPTH : 1, 8>), grid, dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((attn_kernel<BITS, R, NT, DEPTH, 4>), grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -568,7 +573,7 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   const int64_t units = (int64_t)B * Hkv * a.row_tiles;
   PBS_REQUIRE(units < (1 << 22), "pbs_paged_attn_fwd: too many query rows");   // (a grid's threads fit 32 bits)
   // the line of steps that workers share has to fit 32 bits, whatever the lengths turn out to be: a call that may not is not cut
-  if (units * ((int64_t)max_pages * page_size / p.step + 16) > INT32_MAX) p.workers = 0;
+  if (units * ((int64_t)max_pages * page_size / p.step + 16) > INT32_MAX) p.workers = 0, p.waves = 8;
   a.workers = p.workers;
   a.headers = p.workers ? (PagedHeader*)workspace : nullptr;
   a.parts = p.workers ? (float*)((char*)workspace + p.workers * sizeof(PagedHeader)) : nullptr;
@@ -576,18 +581,18 @@ extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void
   if (through_lds(p.rows, kv_bits)) {
     if (const int rc = paged_attn_rows(a, kv_bits, p.rows, st)) return rc;
   } else if (kv_bits == 16) {
-    if (p.rows == 16) launch<16, 1, 1, 1>(a, st);
-    else launch<16, 2, 1, 1>(a, st);
+    if (p.rows == 16) launch<16, 1, 1, 1>(a, p.waves, st);
+    else launch<16, 2, 1, 1>(a, p.waves, st);
   } else if (kv_bits == 8) {
-    if (p.rows == 16) launch<8, 1, 2, 1>(a, st, p.waves);
-    else if (p.rows == 32) launch<8, 2, 1, 1>(a, st);
-    else if (p.rows == 48) launch<8, 3, 1, 1>(a, st);
-    else launch<8, 4, 1, 1>(a, st);
+    if (p.rows == 16) launch<8, 1, 2, 1>(a, p.waves, st);
+    else if (p.rows == 32) launch<8, 2, 1, 1>(a, p.waves, st);
+    else if (p.rows == 48) launch<8, 3, 1, 1>(a, p.waves, st);
+    else launch<8, 4, 1, 1>(a, p.waves, st);
   } else {
-    if (p.rows == 16) launch<4, 1, 2, 2>(a, st);
-    else if (p.rows == 32) launch<4, 2, 2, 1>(a, st);
-    else if (p.rows == 48) launch<4, 3, 2, 1>(a, st);
-    else launch<4, 4, 1, 1>(a, st);
+    if (p.rows == 16) launch<4, 1, 2, 2>(a, p.waves, st);
+    else if (p.rows == 32) launch<4, 2, 2, 1>(a, p.waves, st);
+    else if (p.rows == 48) launch<4, 3, 2, 1>(a, p.waves, st);
+    else launch<4, 4, 1, 1>(a, p.waves, st);
   }
   if (p.workers) {
     const int rows = (int)std::min<int64_t>(p.rows, (int64_t)S * a.G);

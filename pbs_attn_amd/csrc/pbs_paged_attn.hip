@@ -125,7 +125,7 @@ struct Softmax {
   f32x4 o[R][8];
   float m[R];
   // The weights' sums, in 32 bits: as products with ones on the matrix unit (every row of the tile the same, and no sum over lanes), 8 bits of the lane's
-  // own tokens by the vector unit, two at a time (three registers a row tile less: with them the loads go out a step earlier).
+  // own tokens by the vector unit, two at a time: three registers a row tile less (56 rows of 16 sequences 104 -> 93 us; with fewer row tiles the same).
   static constexpr bool LANE_SUMS = BITS == 8;
   typename std::conditional<LANE_SUMS, float, f32x4>::type l[R];
   int seen[R];

@@ -81,3 +81,23 @@ def test_pieces_of_very_different_lengths(dev, lens, Hq, S):
     """Shares that begin and end anywhere in the line of all sequences' steps, in what a piece's beginning counts for among others."""
     f = Filled(Hq, 4 if Hq == 28 else 2, S, lens, page=64, seed=len(lens))
     f.check(f.attn())
+
+
+@pytest.mark.parametrize("Hq,Hkv,S,page", [(8, 2, 1, 64), (8, 2, 1, 32), (28, 4, 5, 128), (28, 4, 9, 32), (8, 2, 40, 32)])
+def test_shares_of_hundreds_of_steps(dev, Hq, Hkv, S, page):
+    """Many sequences that list the pages of one long one: a workgroup goes through more steps than it looks up pages for at once."""
+    n, B = 70000, 160
+    g = torch.Generator(device="cuda").manual_seed(S)
+    slots = (n + page - 1) // page
+    pages = alloc_pages(slots + 1, Hkv, page, "fp8")
+    row = torch.randperm(slots + 1, generator=g, device="cuda")[:slots].int().view(1, -1)
+    ops.paged_append(pages, row, torch.zeros(1, dtype=torch.int32, device="cuda"), _randn(g, 1, Hkv, n, 128), _randn(g, 1, Hkv, n, 128))
+    q = _randn(g, B, Hq, S, 128)
+    past = torch.full((B,), n - S, dtype=torch.int32, device="cuda")
+    past[1::3] -= 20000
+    out = ops.paged_attn(q, pages, row.expand(B, -1).contiguous(), past)
+    k, v = tokens_of(pages, row[0].tolist(), n)
+    for b in (0, 1, 77, 158, 159):
+        m = int(past[b])
+        want, tol = attention(q[b], k[:, :m + S], v[:, :m + S], m, S, 128 ** -0.5)
+        assert ((out[b].double() - want).abs() <= tol).all(), b

@@ -19,7 +19,6 @@ attend to them.
 """
 from __future__ import annotations
 
-import types
 from functools import partial
 from typing import Callable, Optional
 
@@ -226,13 +225,16 @@ def is_model_supported(model):
     return type(model).__name__ in SUPPORTED_MODEL_TYPES
 
 
-def _make_forward(prefill_fn):
+def _patched_class(base, prefill_fn):
+    """A module's class ``base`` with ``prefill_fn`` in its forward.  (A class, and no bound method kept in the module itself: module and method would
+    hold each other, and the weights of a model that is dropped stay on the GPU until the collector's next full pass.)"""
     def new_forward(self, hidden_states, position_embeddings, attention_mask=None, past_key_values=None,
                     cache_position=None, **kwargs):
         return patched_attention_forward(self, hidden_states=hidden_states, position_embeddings=position_embeddings,
                                          attention_mask=attention_mask, past_key_values=past_key_values,
                                          cache_position=cache_position, prefill_fn=prefill_fn, **kwargs)
-    return new_forward
+    return type(base.__name__, (base,), dict(forward=new_forward, original_forward=base.forward, unpatched=base, __module__=base.__module__,
+                                             __qualname__=base.__qualname__, __doc__=base.__doc__))
 
 
 def apply_patch_with_prefill(model, prefill_fn: Optional[Callable] = None, skip_layers: Optional[list] = None):
@@ -256,9 +258,14 @@ def apply_patch_with_prefill(model, prefill_fn: Optional[Callable] = None, skip_
             print(f"  Skipping layer {layer_idx}")
             continue
         attn = layer.self_attn
-        attn.original_forward = attn.forward
+        base = getattr(attn, "unpatched", type(attn))
+        own = vars(attn).pop("forward", None)      # what a hook, or a user who took a patch back, has put there
+        if own is not None:
+            vars(attn).pop("original_forward", None)
+            if getattr(own, "__func__", None) is not base.forward:
+                attn.original_forward = own
         attn.first_patched = patched == 0
-        attn.forward = types.MethodType(_make_forward(prefill_fn), attn)
+        attn.__class__ = _patched_class(base, prefill_fn)
         patched += 1
     print(f"Monkey patch applied. Patched {patched}/{len(layers)} layers.")
     return model

@@ -277,7 +277,9 @@ int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale
  * multiply the values are rounded to bf16 (2^-8 of each at most), and what divides is the sum of the rounded ones.  Finite logits and values give
  * finite results, up to the largest; the smallest (with room for 2^17 tokens in the table, values below 2^-116) lose bits.
  * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
- * positive.  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
+ * positive.  workspace: pbs_paged_attn_workspace_bytes bytes (none where it is 0), 256-byte aligned, rewritten by each call.  The size never
+ * falls as B, S or max_len grow: a workspace for the largest call of a model serves the smaller ones (up to 8.5 MB for 16 query rows of a KV
+ * head, S * Hq / Hkv, 68 MB for more than 64).  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
 size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len);
 int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                        const int32_t* page_table, const int32_t* past_lens, const int32_t* new_lens, void* out, int B, int Hq, int Hkv,

@@ -496,11 +496,16 @@ struct Plan {
   int step;      // its keys
   size_t bytes;
 };
+constexpr int row_tile_of(int64_t rows, int kv_bits) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits != 16 ? 48 : rows <= 64 ? 64 : 128; }
+constexpr size_t worker_bytes(int rows) { return sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(rows); }
+// lengths up to which no call is cut
+constexpr int never_cut(int kv_bits) { return kv_bits == 16 ? 640 : kv_bits == 8 ? 1100 : 1280; }
+
 Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
   max_len = std::min(max_len, PAGED_MAX_TOKENS);
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits != 16 ? 48 : rows <= 64 ? 64 : 128;
+  p.rows = row_tile_of(rows, kv_bits);
   // A cut costs a second launch, 4 us; a workgroup by itself gets 55 GB/s of a bf16 cache.  One sequence, 8 KV heads, uncut against cut: bf16 512
   // tokens 8.7 us against 11.1, 1024 13.3 against 10.2; 4 bits 1024 9.3 against 10.4, 2048 13.0 against 10.7.  Many sequences of 700 tokens in
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
@@ -511,8 +516,8 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // are more than it takes at once and of any lengths: 64 of 10 .. 1000 17.6 against 22.0, .. 2000 33.6 against 35.4, .. 3000 49.0 against 48.3, 64 of
   // 17 .. 8191, 4 KV heads 64.5 against 60.4; five tokens of 128, 4 KV heads, 10 .. 1000 23.2 against 33.3, of 32, 10 .. 2600 26.1 against 24.8.
   const int64_t row_tiles = units * p.rows / 16;   // (4 sequences of 1000, 32 units, 10.3 against 12.4)
-  const int least8 = row_tiles < 48 ? 1100 : row_tiles < 96 ? 1600 : units <= 256 && p.rows == 16 ? 2700 : 2000;
-  const bool cut = max_len > (kv_bits == 16 ? 640 : kv_bits == 8 ? least8 : 1280) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
+  const int least8 = row_tiles < 48 ? never_cut(8) : row_tiles < 96 ? 1600 : units <= 256 && p.rows == 16 ? 2700 : 2000;
+  const bool cut = max_len > (kv_bits == 8 ? least8 : never_cut(kv_bits)) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // One worker of eight waves a compute unit instead of two of four: half as many parts, and no older workgroup that goes ahead.  8 bits, with one row
   // tile and few, long units: 128k tokens of one sequence 58.6 -> 55.9 us, 4 KV heads 39.1 -> 35.8, 32 sequences of 8000 tokens 56.3 -> 54.6.  Not
   // where a worker's share is a step or two (one sequence of 4100 tokens 11.1 -> 11.8, of 16000 15.2 -> 16.0), nor where it crosses from unit to
@@ -526,8 +531,19 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // against 14.3 with four, five tokens of 32 sequences of 1000, 4 KV heads, 17.7 against 19.4; but one sequence of 27 tokens 6.2 against 5.8, of 500 7.8
   // against 7.1, 128 of 500 40.0 against 30.0.
   if (!cut && !through_lds(p.rows, kv_bits)) p.waves = kv_bits == 8 && (units > 256 || max_len <= (p.rows == 16 ? 1000 : 500)) ? 4 : 8;
-  p.bytes = p.workers * (sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(p.rows));
+  p.bytes = p.workers * worker_bytes(p.rows);
   return p;
+}
+
+// What holds every call with these heads and at most these sequences, new tokens and lengths: a row tile's rows, the row tiles and the steps of
+// four waves grow with each of them, and a plan has no more workers than that, though it may have fewer or none.
+size_t workspace_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
+  max_len = std::min(max_len, PAGED_MAX_TOKENS);
+  if (max_len <= never_cut(kv_bits)) return 0;
+  const int64_t rows = (int64_t)S * (Hq / Hkv);
+  const int tile = row_tile_of(rows, kv_bits), step = step_of(tile, kv_bits);
+  const int64_t steps = (int64_t)B * ((rows + tile - 1) / tile) * Hkv * ((max_len + step - 1) / step);
+  return std::min<int64_t>(PAGED_WORKERS, (steps + 7) / 8 * 8) * worker_bytes(tile);
 }
 
 // NT tiles a wave and step, DEPTH steps ahead; with eight waves several row tiles leave each half the registers.
@@ -542,7 +558,7 @@ void launch(const PagedAttnArgs& a, int waves, hipStream_t stream) {
 
 extern "C" size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || S <= 0 || Hq < Hkv || max_len <= 0) return 0;
-  return plan_of(B, Hq, Hkv, S, kv_bits, max_len).bytes;
+  return workspace_of(B, Hq, Hkv, S, kv_bits, max_len);
 }
 
 extern "C" int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,

@@ -257,7 +257,9 @@ int pbs_rope_qk(const void* q, const void* k, const void* cos, const void* sin, 
  * pbs_paged_append: rotary embedding of q (B, Hq, S, 128) and k (B, Hkv, S, 128) in fp32 with one rounding to bf16 (cos and sin as in
  * pbs_rope_qk; both null: no rotation), and k and v into the pages: row i < new_lens[b] at token past_lens[b] + i.  q with q_out, or both
  * null.  k_out (null: not wanted) receives the rotated k.  q_out, k_out: contiguous, head-major, all S rows.  Sequences that share a page
- * may read it, and at most one of them writes it.  Takes the place of pbs_attn/patch/huggingface.py:169-241 (embedding, then the
+ * may read it, and at most one of them writes it.  In 8 bits that one rewrites the block of 32 tokens that it adds to, older tokens' codes and
+ * exponent included, in separate stores: calls that read such a block for another sequence are ordered before the append or behind it (one
+ * stream, or an event), where with 16 and 4 bits they may run beside it, and find its tokens rounded anew behind it.  Takes the place of pbs_attn/patch/huggingface.py:169-241 (embedding, then the
  * cache's own update). */
 int pbs_paged_append(const void* q, const void* k, const void* v, const void* cos, const void* sin, void* q_out, void* k_out, void* k_pages,
                      void* v_pages, void* k_scale, void* v_scale, const int32_t* page_table, const int32_t* past_lens,

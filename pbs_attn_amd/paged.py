@@ -22,7 +22,8 @@ class KVPages:
     bf16: ``k`` (pages, heads, P, 128), ``v`` (pages, heads, P / 8, 128, 8) with the eight tokens of a channel side by side.
 
     8 bits (``k`` and ``v`` float8_e4m3fn): their layouts as in bf16, and a power of two for 32 tokens of a head, as its exponent + 127:
-    ``k_scale``, ``v_scale`` (pages, heads, P / 32) uint8.
+    ``k_scale``, ``v_scale`` (pages, heads, P / 32) uint8.  Tokens that are appended to a block of 32 may take its power up, and those that it
+    holds are then rounded anew: no call reads the block meanwhile, for a sequence that shares its page either.
 
     4 bits (``k_scale`` and ``v_scale`` given): uint8, two e2m1 codes a byte, the even channel in the low half: ``k`` (pages, heads, P, 64),
     ``v`` (pages, heads, P / 4, 16, 4, 4) = (token / 4, channel / 8, token % 4, byte), and a power of two for 32 channels of a token, as its

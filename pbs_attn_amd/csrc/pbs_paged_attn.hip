@@ -7,7 +7,7 @@
 // Here: up to 32 rows of a bf16 cache, up to 64 of an 8- or 4-bit one; pbs_paged_rows.hip and pbs_paged_rows8.hip take more.  Bound by memory, so the waves of a workgroup split
 // the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order and nothing is shared
 // but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
-// parts), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
+// parts; in 8 bits, where few long sequences have one row tile, 256 by workgroups of eight waves), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
 // 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their
 // time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 13 registers of a wave
 // go to scratch memory, 20 with eight waves.)  In 8 bits 128k tokens take 57 us (5.2 TB/s in this launch, then a join of 5 us; reading as much and
@@ -498,8 +498,8 @@ struct Plan {
 };
 constexpr int row_tile_of(int64_t rows, int kv_bits) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && kv_bits != 16 ? 48 : rows <= 64 ? 64 : 128; }
 constexpr size_t worker_bytes(int rows) { return sizeof(PagedHeader) + 2 * sizeof(float) * paged_slot_floats(rows); }
-// lengths up to which no call is cut
-constexpr int never_cut(int kv_bits) { return kv_bits == 16 ? 640 : kv_bits == 8 ? 1100 : 1280; }
+// lengths up to which no call with row tiles of `rows` is cut
+constexpr int never_cut(int kv_bits, int rows) { return kv_bits == 16 ? 640 : kv_bits == 4 ? 1280 : through_lds(rows, 8) ? 950 : 1100; }
 
 Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   Plan p;
@@ -511,13 +511,18 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
   // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  // 8 bits, uncut against cut: one sequence of 700 tokens 8.1 us against 10.6, 1003 10.2 against 10.2, 1300 11.9 against 10.1; where whole units fill half
-  // the chip longer ones too: 16 of 2000 16.2 against 18.9, of 3000 25.0 against 23.7, 8 of 1300 12.8 against 13.8, of 3000 20.1 against 18.1; where they
-  // are more than it takes at once and of any lengths: 64 of 10 .. 1000 17.6 against 22.0, .. 2000 33.6 against 35.4, .. 3000 49.0 against 48.3, 64 of
-  // 17 .. 8191, 4 KV heads 64.5 against 60.4; five tokens of 128, 4 KV heads, 10 .. 1000 23.2 against 33.3, of 32, 10 .. 2600 26.1 against 24.8.
-  const int64_t row_tiles = units * p.rows / 16;   // (4 sequences of 1000, 32 units, 10.3 against 12.4)
-  const int least8 = row_tiles < 48 ? never_cut(8) : row_tiles < 96 ? 1600 : units <= 256 && p.rows == 16 ? 2700 : 2000;
-  const bool cut = max_len > (kv_bits == 8 ? least8 : never_cut(kv_bits)) && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
+  // 8 bits: a cut gains more the longer the units are, and less the more of them there are; the lengths from which it is faster lie near a line for each
+  // kernel.  us, uncut against cut, all sequences of that length (in brackets 10 tokens up to it):
+  //   16 rows    8 units 1250 11.5, 12.1; 1300 12.4, 11.8     32 1250 11.9, 13.0 (11.8, 11.5); 1400 13.0, 12.9 (12.9, 11.5)
+  //              64 1500 15.0, 14.8 (13.2, 11.9); 1800 17.7, 18.2 (15.9, 14.6)     128 2000 19.6, 22.5 (18.0, 19.0); 2400 22.1, 23.5 (20.9, 19.5)
+  //              256 2600 30.1, 34.4 (23.5, 25.4); 3300 36.9, 41.2 (27.8, 26.7)     512 2800 59.4, 62.6 (43.4, 43.2); 3300 70.5, 73.6 (47.1, 45.6)
+  //   48 rows    32 1100 17.6, 18.4; 1300 19.1, 18.9     64 1600 21.9, 23.8 (20.3, 21.3); 2000 26.0, 24.4     128 2000 26.8, 34.1 (25.4, 25.0);
+  //              2400 27.8, 31.3 (26.8, 27.2)     256 3300 43.0, 52.4 (35.9, 38.5); the line costs 4 units of 1000 tokens 2.7: 17.0, 14.3
+  //   by LDS     32 units 1000 29, 37; 1200 33, 30     64 1000 31, 40; 1400 40, 34     128 1400 38, 43; 1800 47, 47     176 1600 43, 47; 2000 54, 51
+  //              256 1800 55, 58; 2200 63, 63     512 4000 123, 125; the line costs 8 units of 800 tokens 9: 24, 15
+  const int64_t least8 = never_cut(8, p.rows) + units * (through_lds(p.rows, 8) ? 5 : 8);
+  const int64_t least = kv_bits == 8 ? std::min<int64_t>(least8, 3300) : never_cut(kv_bits, p.rows);
+  const bool cut = max_len > least && (!through_lds(p.rows, kv_bits) || units < 4 * PAGED_WORKERS);
   // One worker of eight waves a compute unit instead of two of four: half as many parts, and no older workgroup that goes ahead.  8 bits, with one row
   // tile and few, long units: 128k tokens of one sequence 58.6 -> 55.9 us, 4 KV heads 39.1 -> 35.8, 32 sequences of 8000 tokens 56.3 -> 54.6.  Not
   // where a worker's share is a step or two (one sequence of 4100 tokens 11.1 -> 11.8, of 16000 15.2 -> 16.0), nor where it crosses from unit to
@@ -527,10 +532,11 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // (no more workers than there is work for)
   const int64_t steps = units * ((max_len + p.step - 1) / p.step);
   p.workers = cut ? (int)std::min<int64_t>(PAGED_WORKERS * 4 / p.waves, steps + 7) / 8 * 8 : 0;
-  // Whole units have eight waves each where a compute unit has no second one to run beside it and a few steps to share: 8 bits, 16 sequences of 1500 tokens 13.7 us
-  // against 14.3 with four, five tokens of 32 sequences of 1000, 4 KV heads, 17.7 against 19.4; but one sequence of 27 tokens 6.2 against 5.8, of 500 7.8
-  // against 7.1, 128 of 500 40.0 against 30.0.
-  if (!cut && !through_lds(p.rows, kv_bits)) p.waves = kv_bits == 8 && (units > 256 || max_len <= (p.rows == 16 ? 1000 : 500)) ? 4 : 8;
+  // Whole units have eight waves each.  8 bits: only where every compute unit has one at most and four waves would go more than four steps.  us, four
+  // against eight: 16 rows, 8 units, 500 tokens 7.0, 7.7, 1000 10.5, 10.7, 1100 11.9, 11.0; 128 units 500 8.9, 9.2, 1000 13.0, 13.2, 1100 14.6, 13.4;
+  // 256 units 1000 16.0, 16.1, 1100 17.4, 16.8; 512 units, two of which run beside each other, 1100 26.8, 30.6.  48 rows, 64 units, 500 14.6, 14.6,
+  // 700 17.0, 16.4; 256 units 500 17.1, 17.2, 700 19.9, 19.4; 512 units 700 26.4, 36.0.  64 rows, 64 units, 500 16.4, 17.4, 700 19.2, 19.3, 800 20.8, 19.5.
+  if (!cut && !through_lds(p.rows, kv_bits)) p.waves = kv_bits == 8 && (units > 256 || max_len <= 4 * step_of(p.rows, 8)) ? 4 : 8;
   p.bytes = p.workers * worker_bytes(p.rows);
   return p;
 }
@@ -539,10 +545,10 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
 // four waves grow with each of them, and a plan has no more workers than that, though it may have fewer or none.
 size_t workspace_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   max_len = std::min(max_len, PAGED_MAX_TOKENS);
-  if (max_len <= never_cut(kv_bits)) return 0;
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   const int tile = row_tile_of(rows, kv_bits), step = step_of(tile, kv_bits);
-  const int64_t steps = (int64_t)B * ((rows + tile - 1) / tile) * Hkv * ((max_len + step - 1) / step);
+  if (max_len <= never_cut(kv_bits, tile)) return 0;
+  const int64_t units = std::min<int64_t>(PAGED_WORKERS, (int64_t)B * ((rows + tile - 1) / tile) * Hkv), steps = units * ((max_len + step - 1) / step);
   return std::min<int64_t>(PAGED_WORKERS, (steps + 7) / 8 * 8) * worker_bytes(tile);
 }
 

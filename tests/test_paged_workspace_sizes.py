@@ -54,7 +54,7 @@ def test_the_size_holds_what_a_call_asks_for(bits):
     scales = {} if bits == 16 else dict(ks=FAKE, vs=FAKE)
     for _ in range(1500):
         Hq, Hkv = rng.choice(HEADS)
-        B, S, n = rng.choice(BATCHES), rng.choice(NEW), rng.choice([x for x in LENGTHS if 2700 < x < 1 << 28])
+        B, S, n = rng.choice(BATCHES), rng.choice(NEW), rng.choice([x for x in LENGTHS if 3300 < x < 1 << 28])
         if B * Hkv * ((S * (Hq // Hkv) + 15) // 16) >= 2048:
             continue
         assert _attn(lib, B=B, Hq=Hq, Hkv=Hkv, S=S, bits=bits, max_len=n, max_pages=1 << 20, size=256, n=0, **scales) == -1

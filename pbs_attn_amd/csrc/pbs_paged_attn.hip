@@ -275,9 +275,9 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   }
   auto one = [&](auto mask, Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
     const int next = t + DEPTH * STRIDE, k0 = t * PAGED_TILE;
-    // (the older waves of a compute unit would finish a third earlier and leave the memory half idle: they go first in every other step only.
-    // 8 bits: 128k tokens of one sequence 58.6 -> 57.3 us, 128 sequences 374 -> 365)
-    if (BITS == 8 && R == 1) {
+    // (the older of a compute unit's two workgroups would finish a third earlier and leave the memory half idle: they go first in every other step only.
+    // 8 bits: 128k tokens of one sequence 58.6 -> 57.3 us, 128 sequences 374 -> 365; a workgroup of eight waves is alone: no difference)
+    if (BITS == 8 && R == 1 && WAVES == 4) {
       if ((blockIdx.x >= gridDim.x / 2) == (step & 1)) __builtin_amdgcn_s_setprio(0);
       else __builtin_amdgcn_s_setprio(2);
     }

@@ -6,8 +6,8 @@ int paged_pool(PagedPool* p, const char* what, const void* k_pages, const void* 
                const int32_t* page_table, int64_t table_sb, int B, int Hkv, int head_dim, int num_pages, int max_pages, int page_size, int kv_bits) {
   PBS_REQUIRE(k_pages && v_pages && page_table, "%s: null tensor pointer", what);
   PBS_REQUIRE(head_dim == PAGED_D, "%s: head_dim must be 128, got %d", what, head_dim);
-  PBS_REQUIRE(kv_bits == 16 || kv_bits == 4 || (kv_bits == 8 && k_scale && v_scale), "%s: a cache of 16 or 4 bits, or of 8 with its scales, got %d", what,
-              kv_bits);
+  PBS_REQUIRE(kv_bits == 16 || kv_bits == 4 || (kv_bits == 8 && k_scale && v_scale), "%s: a cache of 16 or 4 bits, or of 8 with its scales, got %d%s",
+              what, kv_bits, kv_bits == 8 ? " without them" : "");
   PBS_REQUIRE(kv_bits == 16 || (k_scale && v_scale), "%s: a cache of 4 bits needs its scales", what);
   PBS_REQUIRE(page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "%s: pages of 32, 64, 128 or 256 tokens, got %d", what, page_size);
   PBS_REQUIRE(B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535, "%s: bad shape", what);

@@ -259,8 +259,8 @@ int pbs_rope_qk(const void* q, const void* k, const void* cos, const void* sin, 
  * null.  k_out (null: not wanted) receives the rotated k.  q_out, k_out: contiguous, head-major, all S rows.  Sequences that share a page
  * may read it, and at most one of them writes it.  In 8 bits that one rewrites the block of 32 tokens that it adds to, older tokens' codes and
  * exponent included, in separate stores: calls that read such a block for another sequence are ordered before the append or behind it (one
- * stream, or an event), where with 16 and 4 bits they may run beside it, and find its tokens rounded anew behind it.  Takes the place of pbs_attn/patch/huggingface.py:169-241 (embedding, then the
- * cache's own update). */
+ * stream, or an event), where with 16 and 4 bits they may run beside it, and find its tokens rounded anew behind it.  Takes the place of
+ * pbs_attn/patch/huggingface.py:169-241 (embedding, then the cache's own update). */
 int pbs_paged_append(const void* q, const void* k, const void* v, const void* cos, const void* sin, void* q_out, void* k_out, void* k_pages,
                      void* v_pages, void* k_scale, void* v_scale, const int32_t* page_table, const int32_t* past_lens,
                      const int32_t* new_lens, int B, int Hq, int Hkv, int S, int head_dim, int num_pages, int max_pages, int page_size,
@@ -276,12 +276,15 @@ int pbs_paged_read(const void* k_pages, const void* v_pages, const void* k_scale
 /* Attention of the new tokens (appended before) over their sequences: query row i < new_lens[b] of q (B, Hq, S, 128) sees the tokens
  * 0 .. past_lens[b] + i; out (B, Hq, S, 128) with its own strides.  Rows from new_lens[b] on, and rows whose keys weigh nothing, are zeros.
  * What a row does not see does not reach it, infinities and NaN included.  Logits, sums and the largest exponent are fp32; the weights that
- * multiply the values are rounded to bf16 (2^-8 of each at most), and what divides is the sum of the rounded ones.  Finite logits and values give
+ * multiply the values are rounded to bf16 (2^-8 of each at most), and what divides is the sum of the rounded ones.  With 8 and 4 bits a query is
+ * multiplied as two e4m3 numbers a channel and one power of two a row: exact for channels of 2^-14 of the row's largest and more, smaller ones
+ * off by at most 2^-22 of it.  Finite logits and values give
  * finite results, up to the largest; the smallest (with room for 2^17 tokens in the table, values below 2^-116) lose bits.
  * max_len: no sequence has more tokens, the new ones included; it decides how the work is cut, not what is computed.  softmax_scale must be
  * positive.  workspace: pbs_paged_attn_workspace_bytes bytes (none where it is 0), 256-byte aligned, rewritten by each call.  The size never
  * falls as B, S or max_len grow: a workspace for the largest call of a model serves the smaller ones (up to 8.5 MB for 16 query rows of a KV
- * head, S * Hq / Hkv, 68 MB for more than 64).  Takes the place of the module's own forward on a filled cache (called in pbs_attn/patch/huggingface.py:169-241). */
+ * head, S * Hq / Hkv, 68 MB for more than 64).  Takes the place of the module's own forward on a filled cache (called in
+ * pbs_attn/patch/huggingface.py:169-241). */
 size_t pbs_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int S, int head_dim, int kv_bits, int max_len);
 int pbs_paged_attn_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                        const int32_t* page_table, const int32_t* past_lens, const int32_t* new_lens, void* out, int B, int Hq, int Hkv,

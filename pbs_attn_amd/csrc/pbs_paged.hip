@@ -73,9 +73,9 @@ __device__ __forceinline__ uint32_t rotate_pair(uint32_t x, uint32_t y, uint32_t
 // the heads.  Bound by memory, each row in and out once: an 8192-token prompt (32 / 8 heads) into bf16 pages 49 us, 4.5 TB/s.  A single token
 // takes 3.2 us, two round trips to memory.
 //
-// 8 bits: a workgroup has a tile whole, and its scale is the largest magnitude's over the workgroup and what the tile has.  What is there from before the
-// call is read beside the new rows: a round trip less where the scale grows, 4 KB where it does not.  8192 tokens 47.5 us (4.3 TB/s), a single token
-// 4.2 us.
+// 8 bits: a workgroup has a tile whole, and its scale is the largest magnitude's over the workgroup and what the tile has.  What is there from
+// before the call is read beside the new rows: a round trip less where the scale grows, 4 KB where it does not.  8192 tokens 47.5 us (4.3 TB/s), a
+// single token 4.2 us.
 template <int BITS>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int b = blockIdx.z, past = min(max(a.past[b], 0), PAGED_MAX_TOKENS), fresh = a.fresh ? min(max(a.fresh[b], 0), a.S) : a.S;

@@ -238,8 +238,8 @@ struct Rows<16> {
   }
 };
 // For 8- and 4-bit keys the queries are the sum of two e4m3 numbers a channel: the matrix instruction then takes the keys as they lie in memory, with
-// their scales.  A bf16 value has 8 bits, e4m3 4: q = 2^e (hi + lo / 32) with hi = e4m3(q / 2^e) and lo the 4 bits that are left, exact down to 2^-21
-// of the row's largest channel (below it both halves are subnormal and lo is rounded).
+// their scales.  A bf16 value has 8 bits, e4m3 4: q = 2^e (hi + lo / 32) with hi = e4m3(q / 2^e) and lo the 4 bits that are left.  Exact for channels of
+// 2^-14 of the row's largest and more; of smaller ones lo is a multiple of 2^-9, so they are off by at most 2^-22 of the largest.
 template <>
 struct Rows<4> {
   i32x8 hi, lo;

@@ -4,14 +4,16 @@
 // j <= past + i, m the largest exponent so far (one pass: sums are rescaled where it grows).  All query heads of a KV head and several
 // tokens share a tile's rows, row r = (token r / G, head r % G of the group), so a key is read once for all of them.
 //
-// Here: up to 32 rows of a bf16 cache, up to 64 of an 8- or 4-bit one; pbs_paged_rows.hip and pbs_paged_rows8.hip take more.  Bound by memory, so the waves of a workgroup split
-// the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order and nothing is shared
-// but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and more are slower: more
-// parts; in 8 bits, where few long sequences have one row tile, 256 by workgroups of eight waves), and a second launch joins what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of
-// 17 .. 8191 tokens 109 us (5.1), 128 of 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their
-// time, one step of loads ahead, while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 13 registers of a wave
-// go to scratch memory, 20 with eight waves.)  In 8 bits 128k tokens take 57 us (5.2 TB/s in this launch, then a join of 5 us; reading as much and
-// nothing else 44.5), 128 sequences 366 (5.8), 35 rows of 16 sequences 64 (4.4).
+// Here: up to 32 rows of a bf16 cache, up to 64 of an 8- or 4-bit one; pbs_paged_rows.hip and pbs_paged_rows8.hip take more.  Bound by memory, so
+// the waves of a workgroup split the keys and each holds all rows: tiles go from memory into registers in the matrix instruction's operand order
+// and nothing is shared but the sums at the end.  Sequences of any lengths are cut into 512 equal shares (two workgroups a compute unit; 768 and
+// more are slower: more parts; in 8 bits, where few long sequences have one row tile, 256 by workgroups of eight waves), and a second launch joins
+// what was cut.  32 / 8 heads behind 128k tokens in bf16 103 us (5.2 TB/s; uncut 2721), 64 sequences of 17 .. 8191 tokens 109 us (5.1), 128 of
+// 100 .. 16383 in 4 bits 228 us (5.0).  35 rows in 4 bits are not (60 us, 2.3 TB/s): waves wait for 44 % of their time, one step of loads ahead,
+// while the vector unit works 46 % and the matrix unit 28 %.  (Four row tiles in 4 bits, 49 .. 64 rows: 13 registers of a wave go to scratch
+// memory, 20 with eight waves.)  In 8 bits 128k tokens take 57 us (5.2 TB/s in this launch, then a join of 5 us; reading as much and nothing else
+// 44.5), 128 sequences 366 (5.8), 35 rows of 16 sequences 64 (4.4); 49 .. 64 rows of those 83, with 9 registers of a wave in scratch memory ahead
+// of the steps and behind them, none in a step.
 #include "pbs_paged_attn.h"
 #include "../../include/pbs_hip.h"   // the definitions below are checked against the public declarations
 #include <math.h>
@@ -22,8 +24,8 @@ namespace {
 
 constexpr int O_PITCH = PAGED_D + 4;
 
-// V^T operands: d's holds eight tokens (8 g ..) of channel 16 d + n, of 8-bit pages of channel 32 (d / 2) + 2 n + d % 2, of 4-bit pages of channel 8 n + d; here d = 2 c and 2 c + 1.  `held` of the
-// eight are there.
+// V^T operands: d's holds eight tokens (8 g ..) of channel 16 d + n, of 8-bit pages of channel 32 (d / 2) + 2 n + d % 2, of 4-bit pages of channel
+// 8 n + d; here d = 2 c and 2 c + 1.  `held` of the eight are there.
 template <bool TAIL>
 __device__ __forceinline__ void values(const Tile<16>& t, int c, int held, bf16x8 (&v)[2]) {
 #pragma unroll
@@ -124,8 +126,9 @@ struct Softmax {
   RowsLds* lds;
   f32x4 o[R][8];
   float m[R];
-  // The weights' sums, in 32 bits: as products with ones on the matrix unit (every row of the tile the same, and no sum over lanes), 8 bits of the lane's
-  // own tokens by the vector unit, two at a time: three registers a row tile less (56 rows of 16 sequences 104 -> 93 us; with fewer row tiles the same).
+  // The weights' sums, in 32 bits: as products with ones on the matrix unit (every row of the tile the same, and no sum over lanes), 8 bits of the
+  // lane's own tokens by the vector unit, two at a time: three registers a row tile less (56 rows of 16 sequences 104 -> 93 us; with fewer row
+  // tiles the same).
   static constexpr bool LANE_SUMS = BITS == 8;
   typename std::conditional<LANE_SUMS, float, f32x4>::type l[R];
   int seen[R];
@@ -275,8 +278,8 @@ __device__ __forceinline__ void work(const PagedAttnArgs& a, const PagedUnit& u,
   }
   auto one = [&](auto mask, Tile<BITS> (&tile)[NT], uint32_t& gone) __attribute__((always_inline)) {
     const int next = t + DEPTH * STRIDE, k0 = t * PAGED_TILE;
-    // (the older of a compute unit's two workgroups would finish a third earlier and leave the memory half idle: they go first in every other step only.
-    // 8 bits: 128k tokens of one sequence 58.6 -> 57.3 us, 128 sequences 374 -> 365; a workgroup of eight waves is alone: no difference)
+    // (the older of a compute unit's two workgroups would finish a third earlier and leave the memory half idle: its waves go first in every other
+    // step only.  8 bits: 128k tokens of one sequence 58.6 -> 57.3 us, 128 sequences 374 -> 365; a workgroup of eight waves is alone: no difference)
     if (BITS == 8 && R == 1 && WAVES == 4) {
       if ((blockIdx.x >= gridDim.x / 2) == (step & 1)) __builtin_amdgcn_s_setprio(0);
       else __builtin_amdgcn_s_setprio(2);
@@ -511,8 +514,8 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // bf16, 1300 in 4 bits: 16 of them 12.4 against 16.1 and 12.6 against 16.2, 32 19.6 against 24.7 and 14.5 against 19.0 (the rule's cut costs them
   // this), 64 37.8 against 37.6 and 30.2 against 27.7, 128 72.9 against 71.2 and 58.4 against 49.4.
   const int64_t units = (int64_t)B * ((rows + p.rows - 1) / p.rows) * Hkv;
-  // 8 bits: a cut gains more the longer the units are, and less the more of them there are; the lengths from which it is faster lie near a line for each
-  // kernel.  us, uncut against cut, all sequences of that length (in brackets 10 tokens up to it):
+  // 8 bits: a cut gains more the longer the units are, and less the more of them there are; the lengths from which it is faster lie near a line for
+  // each kernel.  us, uncut against cut, all sequences of that length (in brackets 10 tokens up to it):
   //   16 rows    8 units 1250 11.5, 12.1; 1300 12.4, 11.8     32 1250 11.9, 13.0 (11.8, 11.5); 1400 13.0, 12.9 (12.9, 11.5)
   //              64 1500 15.0, 14.8 (13.2, 11.9); 1800 17.7, 18.2 (15.9, 14.6)     128 2000 19.6, 22.5 (18.0, 19.0); 2400 22.1, 23.5 (20.9, 19.5)
   //              256 2600 30.1, 34.4 (23.5, 25.4); 3300 36.9, 41.2 (27.8, 26.7)     512 2800 59.4, 62.6 (43.4, 43.2); 3300 70.5, 73.6 (47.1, 45.6)
@@ -535,7 +538,8 @@ Plan plan_of(int B, int Hq, int Hkv, int S, int kv_bits, int max_len) {
   // Whole units have eight waves each.  8 bits: only where every compute unit has one at most and four waves would go more than four steps.  us, four
   // against eight: 16 rows, 8 units, 500 tokens 7.0, 7.7, 1000 10.5, 10.7, 1100 11.9, 11.0; 128 units 500 8.9, 9.2, 1000 13.0, 13.2, 1100 14.6, 13.4;
   // 256 units 1000 16.0, 16.1, 1100 17.4, 16.8; 512 units, two of which run beside each other, 1100 26.8, 30.6.  48 rows, 64 units, 500 14.6, 14.6,
-  // 700 17.0, 16.4; 256 units 500 17.1, 17.2, 700 19.9, 19.4; 512 units 700 26.4, 36.0.  64 rows, 64 units, 500 16.4, 17.4, 700 19.2, 19.3, 800 20.8, 19.5.
+  // 700 17.0, 16.4; 256 units 500 17.1, 17.2, 700 19.9, 19.4; 512 units 700 26.4, 36.0.  64 rows, 64 units, 500 16.4, 17.4, 700 19.2, 19.3, 800 20.8,
+  // 19.5.
   if (!cut && !through_lds(p.rows, kv_bits)) p.waves = kv_bits == 8 && (units > 256 || max_len <= 4 * step_of(p.rows, 8)) ? 4 : 8;
   p.bytes = p.workers * worker_bytes(p.rows);
   return p;

@@ -13,10 +13,10 @@
 //    logits of the next's first half    beside   weights of the second half
 //    products of the second half        beside   maxima of the next's first half
 //
-// 1000 new tokens behind 32k (32 / 8 heads) 487 us, 1.12 PFLOP/s (with the logits' two parts counted, 1.68), 500 of two sequences behind up to 16k 212.  By the
-// counters the matrix unit works 51 % of the time and the vector unit 50 %, at 2.25 GHz: an 8-bit matrix instruction keeps the vector unit's issue for
-// about 20 cycles and a bf16 one for 8, so what does run beside them is less than it looks.  With instructions of 32 rows the cycles are 3 % fewer
-// and the clock 6 % lower (2.11 GHz): 533 us for 514 at that time.
+// 1000 new tokens behind 32k (32 / 8 heads) 487 us, 1.12 PFLOP/s (with the logits' two parts counted, 1.68), 500 of two sequences behind up to 16k
+// 212.  By the counters the matrix unit works 51 % of the time and the vector unit 50 %, at 2.25 GHz: an 8-bit matrix instruction keeps the vector
+// unit's issue for about 20 cycles and a bf16 one for 8, so what does run beside them is less than it looks.  With instructions of 32 rows the cycles
+// are 3 % fewer and the clock 6 % lower (2.11 GHz): 533 us for 514 at that time.
 #include "pbs_paged_attn.h"
 #include <math.h>
 
@@ -97,7 +97,8 @@ struct Next {
 
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 // The order within a stretch: after each matrix instruction some of the vector unit's (2), of its exponentials (0x400) and reads from LDS (0x100).
-// (Left to the compiler the matrix instructions end up behind the vector work: 501 us for 493; five vector instructions behind a product 493, three 489.)
+// (Left to the compiler the matrix instructions end up behind the vector work: 501 us for 493; five vector instructions behind a product 493, three
+// 489.)
 __device__ __forceinline__ void beside_logits() {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

@@ -428,8 +428,9 @@ def paged_append(pages, page_table, past_lens, k, v, q=None, cos=None, sin=None,
     Returns (q, k) rotated, contiguous and head-major, all S rows: q (B, Hq, S, 128) where one is given, k with ``want_k``, else None.
 
     Tokens whose page is not in the pool or that lie behind the table are not stored.  At most one sequence may write to a page.  In 8 bits
-    the tokens of a block of 32 (positions 32 t .. 32 t + 31) that are there already are rounded again where new ones take its scale up: whoever reads that block for
-    another sequence, on another stream, has to be ordered before the call or behind it (in bf16 and 4 bits it may run beside it)."""
+    the tokens of a block of 32 (positions 32 t .. 32 t + 31) that are there already are rounded again where new ones take its scale up:
+    whoever reads that block for another sequence, on another stream, has to be ordered before the call or behind it (in bf16 and 4 bits it
+    may run beside it)."""
     done = (_lib._paged_host or _lib.paged_host()).append(pages, page_table, past_lens, k, v, q, cos, sin, new_lens, want_k)
     if done is not None:
         return done

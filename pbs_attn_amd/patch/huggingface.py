@@ -119,7 +119,8 @@ def get_permuted_block_sparse_attn_fwd(
 
 def get_paged_cache(model, batch_size, max_len, page_size=64, form="bf16"):
     """A ``PagedKVCache`` (pbs_attn_amd/patch/paged_cache.py) for a model whose layers are patched: pass it as ``past_key_values``.  ``form``:
-    "bf16", "fp8" for 8 bits or "fp4" for 4.  All layers are on one device."""
+    "bf16", "fp8" for 8 bits or "fp4" for 4.  All layers are on one device.  In 8 bits tokens that are taken off again (``crop``, rejected looked-up
+    tokens) leave their share of the scale to their block of 32."""
     from pbs_attn_amd.patch.paged_cache import PagedKVCache
     k_proj = model.model.layers[0].self_attn.k_proj
     if any(layer.self_attn.k_proj.weight.device != k_proj.weight.device for layer in model.model.layers):

@@ -125,7 +125,8 @@ class _PagedLayer(CacheLayerMixin):
 class PagedKVCache(Cache):
     """Room for ``batch_size`` sequences of up to ``max_len`` tokens of a model with ``config``, in pages of ``page_size`` tokens, bf16,
     8 bits (``form="fp8"``: half of the memory and of a decoding step's traffic) or 4 bits (``form="fp4"``: about a quarter); the first prompt's own
-    attention still sees bf16.
+    attention still sees bf16.  In 8 bits a block of 32 tokens keeps the scale that its largest value asked for, also of tokens that ``crop`` took off
+    again (looked-up or drafted ones that were rejected): those that stay, and those after them, are then held as coarsely as that value made them.
     ``num_kv_heads``: of this process, where it is not the configuration's (tensor parallel)."""
 
     is_paged = True

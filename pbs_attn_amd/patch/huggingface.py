@@ -226,6 +226,10 @@ def is_model_supported(model):
     return type(model).__name__ in SUPPORTED_MODEL_TYPES
 
 
+def _original_forward(base):
+    return getattr(base, "original_forward", base.forward)      # (there where another tool has derived a class from a patched one)
+
+
 def _patched_class(base, prefill_fn):
     """A module's class ``base`` with ``prefill_fn`` in its forward.  (A class, and no bound method kept in the module itself: module and method would
     hold each other, and the weights of a model that is dropped stay on the GPU until the collector's next full pass.)"""
@@ -234,8 +238,8 @@ def _patched_class(base, prefill_fn):
         return patched_attention_forward(self, hidden_states=hidden_states, position_embeddings=position_embeddings,
                                          attention_mask=attention_mask, past_key_values=past_key_values,
                                          cache_position=cache_position, prefill_fn=prefill_fn, **kwargs)
-    return type(base.__name__, (base,), dict(forward=new_forward, original_forward=base.forward, unpatched=base, __module__=base.__module__,
-                                             __qualname__=base.__qualname__, __doc__=base.__doc__))
+    body = dict(forward=new_forward, original_forward=_original_forward(base), unpatched=base)
+    return type(base.__name__, (base,), {**body, "__module__": base.__module__, "__qualname__": base.__qualname__, "__doc__": base.__doc__})
 
 
 def apply_patch_with_prefill(model, prefill_fn: Optional[Callable] = None, skip_layers: Optional[list] = None):
@@ -259,11 +263,11 @@ def apply_patch_with_prefill(model, prefill_fn: Optional[Callable] = None, skip_
             print(f"  Skipping layer {layer_idx}")
             continue
         attn = layer.self_attn
-        base = getattr(attn, "unpatched", type(attn))
+        base = vars(type(attn)).get("unpatched", type(attn))
         own = vars(attn).pop("forward", None)      # what a hook, or a user who took a patch back, has put there
         if own is not None:
             vars(attn).pop("original_forward", None)
-            if getattr(own, "__func__", None) is not base.forward:
+            if getattr(own, "__func__", None) is not _original_forward(base):
                 attn.original_forward = own
         attn.first_patched = patched == 0
         attn.__class__ = _patched_class(base, prefill_fn)

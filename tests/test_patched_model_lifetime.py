@@ -96,3 +96,21 @@ def test_a_forward_that_a_hook_has_put_in_its_place_is_the_original():
         _patch(model)
         calls.clear()
         assert attn.original_forward is hooked and torch.equal(_logits(model, IDS[:, :1]), want) and len(calls) == 1
+
+
+def test_a_class_that_another_tool_has_put_on_top_stays():
+    """As sharding does: a class of the module's class and its own, made after the patch."""
+    model = _tiny("llama")
+    want, one = _logits(model), _logits(model, IDS[:, :1])
+    _patch(model)
+    for layer in model.model.layers:
+        cls = type(layer.self_attn)
+        layer.self_attn.__class__ = type("Sharded" + cls.__name__, (_Mixin, cls), {})
+    for _ in range(2):
+        _patch(model)
+        assert all(isinstance(layer.self_attn, _Mixin) for layer in model.model.layers)
+        assert torch.allclose(_logits(model), want, atol=2e-4) and torch.equal(_logits(model, IDS[:, :1]), one)
+
+
+class _Mixin:
+    pass
